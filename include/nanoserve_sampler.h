@@ -81,8 +81,13 @@ extern "C" {
                                            kept them in index order       */
 #define NS_STATUS_BAD_ROW_ORDER 0x10u   /* row_order[t] outside [0, S): that
                                            slot took row t instead        */
-#define NS_STATUS_BAD_POOL_RANGE 0x20u  /* ns_history_gather / _append: a
-                                           range or slot outside the pool */
+#define NS_STATUS_BAD_POOL_RANGE 0x20u  /* ns_history_gather / _append, ns_paged_history_gather:
+                                           a range, slot or page outside the pool */
+#define NS_STATUS_BAD_TOKEN_ID 0x40u    /* ns_process_logits: a bias id, ns_token_logprobs: a token
+                                           id outside [0, vocab)             */
+#define NS_STATUS_BAD_ROW_RANGE 0x80u   /* ns_process_logits: a row's history or bias range is
+                                           outside its array (or longer than 2^28) */
+#define NS_STATUS_BAD_MASK_ROW 0x100u   /* ns_process_logits: allowed_rows[i] past the masks */
 
 /* One row's sampling parameters (32 bytes, device array [num_rows]).
  * Mirrors nanoserve/config.py:68-79 SamplingParams (temperature :72,
@@ -221,6 +226,140 @@ int ns_history_gather(const int32_t* pool, int64_t pool_size, const int64_t* row
                       int32_t num_rows, int32_t* out_ids, uint32_t* status, void* stream);
 int ns_history_append(int32_t* pool, int64_t pool_size, const int64_t* row_dst, const void* tokens,
                       int32_t tokens_dtype, int32_t num_rows, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------- logits processing
+ *
+ * Arguments of one logits-processing step: the penalties, biases and grammar
+ * masks that a request may ask for on top of the reference's repetition
+ * penalty (sampler.py:31-38).  No counterpart in the reference.
+ *
+ * Row i reads logits row r = sample_indices[i] (or i).  With hist_i =
+ * history_ids[history_offsets[i] .. history_offsets[i+1]), seen(v) = v occurs
+ * in hist_i, and c(v) = how often it occurs at positions >= prompt_lens[i]:
+ *
+ *   x = float(logits[r, v])
+ *   x = x < 0 ? x * rp : x / rp            if seen(v)        (rp: repetition_penalty[i])
+ *   x = x - frequency_penalty[i] * c(v) - presence_penalty[i]   if c(v) > 0
+ *   x = x + bias                           if row i has a bias for v (the last entry for v counts)
+ *   x = -inf                               if row i has a mask whose bit v is 0
+ *
+ * in fp32 whatever the logits' type, rounded to the output's type once.  Row
+ * i's mask is row allowed_rows[i] of `allowed` (none if negative; row i where
+ * allowed_rows is NULL); bit v is bit v % 32 of word v / 32.
+ *
+ * out may be the logits themselves (same address, type and row stride, no
+ * sample_indices): then only the elements that change are written.  Any
+ * other overlap of the two is refused.
+ *
+ * Bad device data is never followed out of bounds: a sample index outside the
+ * logits reads row 0, a history or bias id outside [0, vocab) is skipped, a
+ * range outside its array counts as empty, a mask row past the masks as none;
+ * each sets its NS_STATUS_* bit. */
+typedef struct NsProcessArgs {
+  const void* logits;          /* device [num_logit_rows, row_stride]      */
+  int32_t logits_dtype;        /* NS_DTYPE_*                               */
+  int32_t vocab_size;          /* V                                        */
+  int64_t num_logit_rows;
+  int64_t logits_row_stride;   /* elements between rows (>= 0)             */
+  int32_t num_rows;            /* S                                        */
+  int32_t out_dtype;           /* NS_DTYPE_* (fp32, or the logits' type)   */
+  const int64_t* sample_indices;   /* device [S] or NULL                   */
+  const int64_t* history_offsets;  /* device [S+1] or NULL (no history)    */
+  const int32_t* history_ids;      /* device [num_history_ids]             */
+  int64_t num_history_ids;
+  const int32_t* prompt_lens;      /* device [S] or NULL (all zero)        */
+  const float* repetition_penalty; /* device [S] or NULL (all 1)           */
+  const float* presence_penalty;   /* device [S] or NULL (all 0)           */
+  const float* frequency_penalty;  /* device [S] or NULL (all 0)           */
+  const int64_t* bias_offsets;     /* device [S+1] or NULL (no biases)     */
+  const int32_t* bias_ids;         /* device [num_biases]                  */
+  const float* bias_values;        /* device [num_biases]                  */
+  int64_t num_biases;
+  const int32_t* allowed;          /* device [num_masks, mask_stride] or NULL */
+  int64_t mask_stride;             /* words between masks (>= (V+31)/32)   */
+  int32_t num_masks;
+  int32_t reserved;                /* must be 0                            */
+  const int32_t* allowed_rows;     /* device [S] or NULL (row i: mask i)   */
+  void* out;                       /* device [S, out_row_stride]           */
+  int64_t out_row_stride;          /* elements between rows (>= V)         */
+  uint32_t* status;                /* device [1] or NULL                   */
+} NsProcessArgs;
+
+/* Enqueue one logits-processing step on `stream`: host-side checks only, no
+ * host synchronisation, no allocation, no workspace. */
+int ns_process_logits(const NsProcessArgs* args, void* stream);
+
+/* ---------------------------------------------------------------- log-probabilities
+ *
+ * Row i reads logits row r = sample_indices[i] (or i); x = float(logits[r]),
+ * L = log(sum_v exp(x_v)), t = token_ids[i]:
+ *
+ *   out_logprobs[i]     = x_t - L
+ *   out_ranks[i]        = 1 + #{v : x_v > x_t}
+ *   out_top_ids[i, j], out_top_logprobs[i, j], j < top_n: the top_n largest
+ *                         logits, larger first, equal ones by ascending id,
+ *                         with their x - L
+ *
+ * A row that the sampler's guard makes uniform (a NaN, a +inf, or only -inf:
+ * sampler.py:78-80) has log-probability -log(V) everywhere, all ids tied: rank
+ * 1, top ids 0 .. top_n-1.  A token id outside [0, V) gets NaN and rank 0 and
+ * sets NS_STATUS_BAD_TOKEN_ID; a sample index outside the logits reads row 0
+ * and sets NS_STATUS_BAD_SAMPLE_INDEX.  No counterpart in the reference. */
+#define NS_MAX_TOP_LOGPROBS 32
+typedef struct NsLogprobArgs {
+  const void* logits;          /* device [num_logit_rows, row_stride]      */
+  int32_t logits_dtype;        /* NS_DTYPE_*                               */
+  int32_t vocab_size;          /* V                                        */
+  int64_t num_logit_rows;
+  int64_t logits_row_stride;   /* elements between rows (>= 0)             */
+  int32_t num_rows;            /* S                                        */
+  int32_t ids_dtype;           /* NS_OUT_*: token_ids and out_top_ids      */
+  const int64_t* sample_indices;   /* device [S] or NULL                   */
+  const void* token_ids;           /* device [S]                           */
+  int32_t top_n;                   /* 0 .. min(V, NS_MAX_TOP_LOGPROBS)     */
+  int32_t reserved;                /* must be 0                            */
+  float* out_logprobs;             /* device [S]                           */
+  int32_t* out_ranks;              /* device [S]                           */
+  void* out_top_ids;               /* device [S, top_n] (top_n > 0)        */
+  float* out_top_logprobs;         /* device [S, top_n] (top_n > 0)        */
+  uint32_t* status;                /* device [1] or NULL                   */
+} NsLogprobArgs;
+
+/* Enqueue one log-probability step on `stream`: host-side checks only, no
+ * host synchronisation, no allocation, no workspace. */
+int ns_token_logprobs(const NsLogprobArgs* args, void* stream);
+
+/* ---------------------------------------------------------------- cache pages
+ *
+ * A paged cache is a set of pools that one page table indexes: page p of a
+ * pool is page_bytes bytes at base + p * page_stride (for instance one pool
+ * of token ids, and one of keys and one of values per layer).
+ *
+ * ns_pages_copy: pool[dst[j]] = pool[src[j]] for every pool and every j <
+ * count.  pools, src and dst are HOST arrays, read during the call (inside a
+ * stream capture their values become part of the graph).  A page may be a
+ * source several times; a page outside [0, num_pages), a destination named
+ * twice, or a page that is both source and destination is refused
+ * (NS_ERR_INVALID_ARG) before anything is enqueued.
+ *
+ * ns_paged_history_gather: row r's prior ids out of a pool of int32 pages,
+ *   out_ids[offsets[r] + j] = pool[pages[page_offsets[r] + j / page_size] * page_size + j % page_size]
+ *   for j < offsets[r+1] - offsets[r]: the CSR history_ids of NsSampleArgs
+ *   and NsProcessArgs.  All pointers are device pointers.  An id whose page
+ *   lies outside the row's table, outside pages[num_table_pages] or outside
+ *   the pool becomes -1, ids outside out_ids[num_ids] are not written; both
+ *   set NS_STATUS_BAD_POOL_RANGE. */
+typedef struct NsPagePool {
+  void* base;           /* device                                          */
+  int64_t page_stride;  /* bytes between pages (>= page_bytes)             */
+  int64_t page_bytes;   /* bytes of a page (> 0)                           */
+} NsPagePool;
+
+int ns_pages_copy(const NsPagePool* pools, int32_t num_pools, int64_t num_pages, const int64_t* src,
+                  const int64_t* dst, int64_t count, void* stream);
+int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page_size, const int32_t* pages,
+                            int64_t num_table_pages, const int64_t* page_offsets, const int64_t* offsets,
+                            int32_t num_rows, int32_t* out_ids, int64_t num_ids, uint32_t* status, void* stream);
 
 /* Message for the last non-OK status returned on this host thread. */
 const char* ns_last_error(void);

@@ -10,7 +10,7 @@ class, so callers do not have to switch types.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Optional
+from typing import Dict, Optional
 
 
 @dataclass
@@ -26,3 +26,15 @@ class SamplingParams:
     stop: list = field(default_factory=list)
     ignore_eos: bool = False
     seed: Optional[int] = None
+
+
+@dataclass
+class ExtendedSamplingParams(SamplingParams):
+    """``SamplingParams`` plus what a serving API asks for and the reference does
+    not know (see :func:`process_logits`).  Presence and frequency penalties count
+    the tokens after the request's prompt.  ``logit_bias`` maps token ids to
+    values that are added to their logits; ``-inf`` bans a token."""
+
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None

@@ -1,10 +1,11 @@
-// ns_torch_ops.cpp -- registers torch.ops.nanoserve_b200.sample over the C ABI.
+// ns_torch_ops.cpp -- registers torch.ops.nanoserve_b200.* over the C ABI.
 //
-// A thin adapter: it checks devices/dtypes, turns tensors into raw pointers,
-// fills an NsSampleArgs and calls ns_sample() on the current CUDA stream.
-// No math happens here; the kernel lives in libnanoserve_sampler.so.
+// A thin adapter: each op checks devices/dtypes, turns tensors into raw
+// pointers, fills the argument struct (NsSampleArgs and its like) and calls
+// the C entry point on the current CUDA stream of the tensors' device.
+// No math happens here; the kernels live in libnanoserve_sampler.so.
 //
-// Each (device, stream) gets its own workspace (NsSampleArgs.workspace),
+// ``sample`` alone needs a workspace: each (device, stream) gets its own workspace (NsSampleArgs.workspace),
 // zeroed once when it is allocated through torch's caching allocator and
 // left zero by every call, so calls on different streams never share one.
 // Warm a stream up before capturing a graph on it, so that the graph does
@@ -17,6 +18,7 @@
 
 #include <mutex>
 #include <unordered_map>
+#include <vector>
 
 #include "../../include/nanoserve_sampler.h"
 
@@ -151,6 +153,227 @@ void sample_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample
   TORCH_CHECK(rc == NS_OK, "ns_sample failed (", rc, "): ", ns_last_error());
 }
 
+bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+
+void check_size(const c10::optional<at::Tensor>& t, int64_t n, const char* name) {
+  if (given(t)) TORCH_CHECK(t->numel() == n, name, " must have ", n, " elements, it has ", t->numel());
+}
+
+// fp32 or bf16 rows; returns NS_DTYPE_*
+int32_t check_rows(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.dim() == 2, name, " must be 2-D [rows, vocab]");
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " rows must be contiguous");
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, " must be float32 or bfloat16");
+  TORCH_CHECK(t.size(1) > 0 && t.size(1) <= INT32_MAX, name, " must have between 1 and 2^31 - 1 columns");
+  return t.scalar_type() == at::kFloat ? NS_DTYPE_F32 : NS_DTYPE_BF16;
+}
+
+template <typename T>
+T* opt_data(const c10::optional<at::Tensor>& t) {
+  return static_cast<T*>(const_cast<void*>(opt_ptr(t)));
+}
+
+// process_logits(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
+//   presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows, out, status) -> ()
+void process_logits_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
+                       const c10::optional<at::Tensor>& history_offsets, const c10::optional<at::Tensor>& history_ids,
+                       const c10::optional<at::Tensor>& prompt_lens,
+                       const c10::optional<at::Tensor>& repetition_penalty,
+                       const c10::optional<at::Tensor>& presence_penalty,
+                       const c10::optional<at::Tensor>& frequency_penalty,
+                       const c10::optional<at::Tensor>& bias_offsets, const c10::optional<at::Tensor>& bias_ids,
+                       const c10::optional<at::Tensor>& bias_values, const c10::optional<at::Tensor>& allowed,
+                       const c10::optional<at::Tensor>& allowed_rows, at::Tensor& out,
+                       const c10::optional<at::Tensor>& status) {
+  NsProcessArgs a = {};
+  a.logits_dtype = check_rows(logits, "logits");
+  a.out_dtype = check_rows(out, "out");
+  const at::Device dev = logits.device();
+  c10::cuda::CUDAGuard guard(dev);
+  TORCH_CHECK(out.device() == dev, "out must be on ", dev);
+  const int64_t S = out.size(0), V = logits.size(1);
+  TORCH_CHECK(S <= INT32_MAX, "out has too many rows");
+  TORCH_CHECK(out.size(1) == V, "out must have the logits' columns");
+  TORCH_CHECK(given(sample_indices) || logits.size(0) == S, "out must have one row per row of logits");
+  check_opt(sample_indices, dev, "sample_indices", at::kLong);
+  check_opt(history_offsets, dev, "history_offsets", at::kLong);
+  check_opt(history_ids, dev, "history_ids", at::kInt);
+  check_opt(prompt_lens, dev, "prompt_lens", at::kInt);
+  check_opt(repetition_penalty, dev, "repetition_penalty", at::kFloat);
+  check_opt(presence_penalty, dev, "presence_penalty", at::kFloat);
+  check_opt(frequency_penalty, dev, "frequency_penalty", at::kFloat);
+  check_opt(bias_offsets, dev, "bias_offsets", at::kLong);
+  check_opt(bias_ids, dev, "bias_ids", at::kInt);
+  check_opt(bias_values, dev, "bias_values", at::kFloat);
+  check_opt(allowed_rows, dev, "allowed_rows", at::kInt);
+  check_opt(status, dev, "status", at::kInt);
+  check_size(sample_indices, S, "sample_indices");
+  check_size(history_offsets, S + 1, "history_offsets");
+  check_size(prompt_lens, S, "prompt_lens");
+  check_size(repetition_penalty, S, "repetition_penalty");
+  check_size(presence_penalty, S, "presence_penalty");
+  check_size(frequency_penalty, S, "frequency_penalty");
+  check_size(bias_offsets, S + 1, "bias_offsets");
+  check_size(allowed_rows, S, "allowed_rows");
+  check_size(status, 1, "status");
+  TORCH_CHECK(given(history_offsets) == given(history_ids), "history_offsets and history_ids go together");
+  TORCH_CHECK(given(bias_offsets) == given(bias_ids) && given(bias_ids) == given(bias_values),
+              "bias_offsets, bias_ids and bias_values go together");
+  if (given(bias_ids)) check_size(bias_values, bias_ids->numel(), "bias_values");
+  TORCH_CHECK(given(allowed) || !given(allowed_rows), "allowed_rows given without allowed");
+  if (given(allowed)) {
+    TORCH_CHECK(allowed->is_cuda() && allowed->device() == dev, "allowed must be on ", dev);
+    TORCH_CHECK(allowed->scalar_type() == at::kInt && allowed->dim() == 2 && allowed->size(1) >= (V + 31) / 32 &&
+                    allowed->stride(1) == 1,
+                "allowed must be int32 [masks, at least ", (V + 31) / 32, " words], its rows contiguous");
+    TORCH_CHECK(allowed->size(0) <= INT32_MAX, "allowed has too many rows");
+    TORCH_CHECK(allowed->size(0) <= 1 || allowed->stride(0) >= (V + 31) / 32, "allowed's rows overlap");
+    TORCH_CHECK(given(allowed_rows) || allowed->size(0) == S, "allowed must have one row per row, or allowed_rows");
+    a.allowed = static_cast<const int32_t*>(allowed->data_ptr());
+    a.mask_stride = std::max<int64_t>(allowed->stride(0), (V + 31) / 32);
+    a.num_masks = (int32_t)allowed->size(0);
+  }
+  if (S == 0) return;
+  a.logits = logits.data_ptr();
+  a.vocab_size = (int32_t)V;
+  a.num_logit_rows = logits.size(0);
+  a.logits_row_stride = logits.size(0) == 1 ? V : logits.stride(0);
+  a.num_rows = (int32_t)S;
+  a.sample_indices = opt_data<const int64_t>(sample_indices);
+  a.history_offsets = opt_data<const int64_t>(history_offsets);
+  a.history_ids = opt_data<const int32_t>(history_ids);
+  a.num_history_ids = given(history_ids) ? history_ids->numel() : 0;
+  a.prompt_lens = opt_data<const int32_t>(prompt_lens);
+  a.repetition_penalty = opt_data<const float>(repetition_penalty);
+  a.presence_penalty = opt_data<const float>(presence_penalty);
+  a.frequency_penalty = opt_data<const float>(frequency_penalty);
+  a.bias_offsets = opt_data<const int64_t>(bias_offsets);
+  a.bias_ids = opt_data<const int32_t>(bias_ids);
+  a.bias_values = opt_data<const float>(bias_values);
+  a.num_biases = given(bias_ids) ? bias_ids->numel() : 0;
+  a.allowed_rows = opt_data<const int32_t>(allowed_rows);
+  a.out = out.data_ptr();
+  a.out_row_stride = S == 1 ? V : out.stride(0);
+  a.status = opt_data<uint32_t>(status);
+  const int rc = ns_process_logits(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  TORCH_CHECK(rc == NS_OK, "ns_process_logits failed (", rc, "): ", ns_last_error());
+}
+
+// token_logprobs(logits, sample_indices, token_ids, out_logprobs, out_ranks, out_top_ids, out_top_logprobs, status) -> ()
+void token_logprobs_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
+                       const at::Tensor& token_ids, at::Tensor& out_logprobs, at::Tensor& out_ranks,
+                       at::Tensor& out_top_ids, at::Tensor& out_top_logprobs,
+                       const c10::optional<at::Tensor>& status) {
+  NsLogprobArgs a = {};
+  a.logits_dtype = check_rows(logits, "logits");
+  const at::Device dev = logits.device();
+  c10::cuda::CUDAGuard guard(dev);
+  check_cuda(token_ids, dev, "token_ids");
+  TORCH_CHECK(token_ids.scalar_type() == at::kLong || token_ids.scalar_type() == at::kInt,
+              "token_ids must be int64 or int32");
+  const int64_t S = token_ids.numel(), V = logits.size(1);
+  TORCH_CHECK(S <= INT32_MAX, "token_ids has too many elements");
+  TORCH_CHECK(given(sample_indices) || logits.size(0) == S, "token_ids must have one element per row of logits");
+  check_opt(sample_indices, dev, "sample_indices", at::kLong);
+  check_size(sample_indices, S, "sample_indices");
+  check_opt(status, dev, "status", at::kInt);
+  check_size(status, 1, "status");
+  check_opt(out_logprobs, dev, "out_logprobs", at::kFloat);
+  check_size(out_logprobs, S, "out_logprobs");
+  check_opt(out_ranks, dev, "out_ranks", at::kInt);
+  check_size(out_ranks, S, "out_ranks");
+  check_opt(out_top_ids, dev, "out_top_ids", token_ids.scalar_type());
+  check_opt(out_top_logprobs, dev, "out_top_logprobs", at::kFloat);
+  TORCH_CHECK(out_top_ids.dim() == 2 && out_top_ids.size(0) == S, "out_top_ids must be [rows, top_n]");
+  const int64_t n = out_top_ids.size(1);
+  TORCH_CHECK(n <= NS_MAX_TOP_LOGPROBS && n <= V, "top_n must be at most min(vocab, ", NS_MAX_TOP_LOGPROBS, ")");
+  check_size(out_top_logprobs, S * n, "out_top_logprobs");
+  if (S == 0) return;
+  a.logits = logits.data_ptr();
+  a.vocab_size = (int32_t)V;
+  a.num_logit_rows = logits.size(0);
+  a.logits_row_stride = logits.size(0) == 1 ? V : logits.stride(0);
+  a.num_rows = (int32_t)S;
+  a.ids_dtype = token_ids.scalar_type() == at::kLong ? NS_OUT_I64 : NS_OUT_I32;
+  a.sample_indices = opt_data<const int64_t>(sample_indices);
+  a.token_ids = token_ids.data_ptr();
+  a.top_n = (int32_t)n;
+  a.out_logprobs = static_cast<float*>(out_logprobs.data_ptr());
+  a.out_ranks = static_cast<int32_t*>(out_ranks.data_ptr());
+  a.out_top_ids = out_top_ids.data_ptr();
+  a.out_top_logprobs = static_cast<float*>(out_top_logprobs.data_ptr());
+  a.status = opt_data<uint32_t>(status);
+  const int rc = ns_token_logprobs(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  TORCH_CHECK(rc == NS_OK, "ns_token_logprobs failed (", rc, "): ", ns_last_error());
+}
+
+// copy_pages(pools, src, dst) -> (): src and dst are CPU int64 lists of pages
+void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor& dst) {
+  TORCH_CHECK(src.device().is_cpu() && dst.device().is_cpu() && src.scalar_type() == at::kLong &&
+                  dst.scalar_type() == at::kLong && src.is_contiguous() && dst.is_contiguous(),
+              "src and dst must be contiguous int64 CPU tensors");
+  TORCH_CHECK(src.numel() == dst.numel(), "src and dst must have the same number of pages");
+  if (pools.empty()) return;
+  const at::Device dev = pools[0].device();
+  TORCH_CHECK(dev.is_cuda(), "pools must be CUDA tensors");
+  const int64_t num_pages = pools[0].dim() > 0 ? pools[0].size(0) : 0;
+  std::vector<NsPagePool> p;
+  p.reserve(pools.size());
+  for (const at::Tensor& t : pools) {
+    TORCH_CHECK(t.is_cuda() && t.device() == dev, "pools must be on one device");
+    TORCH_CHECK(t.dim() > 0 && t.size(0) == num_pages, "pools must have the same number of pages (dimension 0)");
+    int64_t elems = 1;
+    bool packed = true;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+      packed = packed && (t.size(d) == 1 || t.stride(d) == elems);
+      elems *= t.size(d);
+    }
+    TORCH_CHECK(packed, "each page of a pool must be contiguous");
+    const int64_t stride = num_pages > 1 ? t.stride(0) : elems;
+    TORCH_CHECK(num_pages <= 1 || stride >= elems, "a pool's pages overlap");
+    if (elems == 0 || num_pages == 0) continue;
+    p.push_back({t.data_ptr(), stride * (int64_t)t.element_size(), elems * (int64_t)t.element_size()});
+  }
+  if (p.empty()) {
+    TORCH_CHECK(num_pages > 0 || src.numel() == 0, "page outside an empty pool");
+    return;
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  const int rc = ns_pages_copy(p.data(), (int32_t)p.size(), num_pages, static_cast<const int64_t*>(src.data_ptr()),
+                               static_cast<const int64_t*>(dst.data_ptr()), src.numel(),
+                               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  TORCH_CHECK_VALUE(rc != NS_ERR_INVALID_ARG, ns_last_error());
+  TORCH_CHECK(rc == NS_OK, "ns_pages_copy failed (", rc, "): ", ns_last_error());
+}
+
+// paged_history_gather(pool, pages, page_offsets, history_offsets, out, status) -> ()
+void paged_history_gather_op(const at::Tensor& pool, const at::Tensor& pages, const at::Tensor& page_offsets,
+                             const at::Tensor& history_offsets, at::Tensor& out,
+                             const c10::optional<at::Tensor>& status) {
+  TORCH_CHECK(pool.is_cuda(), "pool must be a CUDA tensor");
+  const at::Device dev = pool.device();
+  c10::cuda::CUDAGuard guard(dev);
+  check_opt(pool, dev, "pool", at::kInt);
+  check_opt(pages, dev, "pages", at::kInt);
+  check_opt(page_offsets, dev, "page_offsets", at::kLong);
+  check_opt(history_offsets, dev, "history_offsets", at::kLong);
+  check_opt(out, dev, "out", at::kInt);
+  check_opt(status, dev, "status", at::kInt);
+  check_size(status, 1, "status");
+  TORCH_CHECK(pool.dim() == 2 && pool.size(1) > 0 && pool.size(1) <= INT32_MAX, "pool must be [pages, page_size]");
+  TORCH_CHECK(history_offsets.numel() >= 1 && history_offsets.numel() <= INT32_MAX,
+              "history_offsets must have rows+1 elements");
+  TORCH_CHECK(page_offsets.numel() == history_offsets.numel(), "page_offsets must have rows+1 elements");
+  const int rc = ns_paged_history_gather(
+      static_cast<const int32_t*>(pool.data_ptr()), pool.size(0), (int32_t)pool.size(1),
+      static_cast<const int32_t*>(pages.data_ptr()), pages.numel(), static_cast<const int64_t*>(page_offsets.data_ptr()),
+      static_cast<const int64_t*>(history_offsets.data_ptr()), (int32_t)(history_offsets.numel() - 1),
+      static_cast<int32_t*>(out.data_ptr()), out.numel(), opt_data<uint32_t>(status),
+      c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  TORCH_CHECK(rc == NS_OK, "ns_paged_history_gather failed (", rc, "): ", ns_last_error());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(nanoserve_b200, m) {
@@ -159,6 +382,24 @@ TORCH_LIBRARY(nanoserve_b200, m) {
       "Tensor? history_ids, Tensor? uniforms, int philox_seed, int philox_offset, int row_offset, "
       "Tensor(a!) out, Tensor(b!)? out_penalized, Tensor(c!)? out_filtered, Tensor(d!)? out_probs, "
       "Tensor(e!)? status, Tensor? row_order=None, int kernel=0) -> ()");
+  m.def(
+      "process_logits(Tensor logits, Tensor? sample_indices, Tensor? history_offsets, Tensor? history_ids, "
+      "Tensor? prompt_lens, Tensor? repetition_penalty, Tensor? presence_penalty, Tensor? frequency_penalty, "
+      "Tensor? bias_offsets, Tensor? bias_ids, Tensor? bias_values, Tensor? allowed, Tensor? allowed_rows, "
+      "Tensor(a!) out, Tensor(b!)? status=None) -> ()");
+  m.def(
+      "token_logprobs(Tensor logits, Tensor? sample_indices, Tensor token_ids, Tensor(a!) out_logprobs, "
+      "Tensor(b!) out_ranks, Tensor(c!) out_top_ids, Tensor(d!) out_top_logprobs, Tensor(e!)? status=None) -> ()");
+  m.def("copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst) -> ()");
+  m.def(
+      "paged_history_gather(Tensor pool, Tensor pages, Tensor page_offsets, Tensor history_offsets, "
+      "Tensor(a!) out, Tensor(b!)? status=None) -> ()");
 }
 
-TORCH_LIBRARY_IMPL(nanoserve_b200, CUDA, m) { m.impl("sample", &sample_op); }
+TORCH_LIBRARY_IMPL(nanoserve_b200, CUDA, m) {
+  m.impl("sample", &sample_op);
+  m.impl("process_logits", &process_logits_op);
+  m.impl("token_logprobs", &token_logprobs_op);
+  m.impl("copy_pages", &copy_pages_op);
+  m.impl("paged_history_gather", &paged_history_gather_op);
+}

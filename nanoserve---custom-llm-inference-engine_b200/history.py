@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from . import _cabi, packing
-from .sampler import Sampler, _Staging, _sm_count
+from .sampler import Sampler, _Staging, _sm_count, upload_parts
 
 
 class RegionAllocator:
@@ -87,7 +87,90 @@ def plan_step(params: Sequence, starts: np.ndarray, lengths: np.ndarray, vocab: 
     return rows, offsets, src
 
 
-class HistoryStore:
+class StoreSampling:
+    """What the history stores share: one step over histories on the device.
+
+    A store has ``length`` and ``prompt_length`` of a request,
+    ``_history_parts(handles, lens)`` (host arrays that say where the first
+    ``lens[i]`` ids of each request are) and ``_history_ids(parts, offsets, ids)``
+    (those ids in CSR order, given the arrays on the device)."""
+
+    def pack(self, params: Sequence, handles: Sequence[int], sms: Optional[int] = None):
+        """Device (row_params, offsets, ids, order) for ``Sampler.sample_packed``."""
+        if len(handles) != len(params):
+            raise ValueError(f"{len(handles)} handles for {len(params)} sampling params")
+        lengths = np.fromiter((self.length(h) for h in handles), dtype=np.int64, count=len(handles))
+        rows, offsets, _ = plan_step(params, lengths, lengths, self.vocab)
+        lens = np.diff(offsets)
+        total = int(offsets[-1])
+        order = packing.schedule(rows, sms) if sms else None
+        parts = [rows.view(np.uint8), offsets] + ([order] if order is not None else [])
+        n = len(parts)
+        with torch.cuda.device(self.device):
+            up = upload_parts(self._staging, parts + (self._history_parts(handles, lens) if total else []), self.device)
+            order_d = up[2] if order is not None else None
+            if total == 0:
+                return up[0], None, None, order_d
+            return up[0], up[1], self._gathered(up[n:], up[1], total), order_d
+
+    def _gathered(self, parts: Sequence[torch.Tensor], offsets: torch.Tensor, total: int) -> torch.Tensor:
+        if self._ids is None or self._ids.numel() < total:
+            self._ids = torch.empty(max(total, 1 << 16), dtype=torch.int32, device=self.device)
+        ids = self._ids[:total]
+        self._history_ids(parts, offsets, ids)
+        return ids
+
+    def sample(self, sampler: Sampler, logits: torch.Tensor, sampling_params_list: Sequence, handles: Sequence[int],
+               *, append: bool = True, logprobs: Optional[int] = None, allowed: Optional[torch.Tensor] = None,
+               allowed_rows: Optional[torch.Tensor] = None, **kw):
+        """``Sampler.sample`` with the histories taken from this store; the
+        sampled ids are appended to the requests' histories (``append``).
+        Presence and frequency penalties count the tokens after each request's
+        prompt; ``allowed``, ``allowed_rows`` and ``logprobs`` are ``Sampler.sample``'s.
+        Runs on the store's device (whatever device is current) inside an NVTX
+        range named ``logits+sample`` (nanoserve/engine/engine.py:234)."""
+        if allowed_rows is not None and allowed is None:
+            raise ValueError("allowed_rows given without allowed")
+        torch.cuda.nvtx.range_push("logits+sample")
+        try:
+            with torch.cuda.device(self.device):
+                if allowed is not None or packing.wants_processing(sampling_params_list):
+                    if len(handles) != len(sampling_params_list):
+                        raise ValueError(f"{len(handles)} handles for {len(sampling_params_list)} sampling params")
+                    out = sampler._sample_processed(
+                        logits, sampling_params_list, _StoreHistories(self, handles),
+                        [self.prompt_length(h) for h in handles], allowed=allowed, allowed_rows=allowed_rows,
+                        logprobs=logprobs, **kw)
+                else:
+                    rp, off, ids, order = self.pack(sampling_params_list, handles, sms=_sm_count(logits.device))
+                    out = sampler.sample_packed(logits, rp, off, ids, row_order=order, **kw)
+                    out = sampler._with_logprobs(out, logits, logprobs, kw.get("sample_indices"))
+                if append:
+                    tokens = out[0] if logprobs is not None else out
+                    self.append(handles, tokens[0] if isinstance(tokens, tuple) else tokens)
+                return out
+        finally:
+            torch.cuda.nvtx.range_pop()
+
+
+class _StoreHistories:
+    """A store's histories, for ``Sampler._sample_processed``."""
+
+    def __init__(self, store: StoreSampling, handles: Sequence[int]):
+        self._store, self._handles = store, handles
+
+    def lens(self) -> np.ndarray:
+        n = len(self._handles)
+        return np.fromiter((self._store.length(h) for h in self._handles), dtype=np.int64, count=n)
+
+    def parts(self, lens: np.ndarray) -> List[np.ndarray]:
+        return self._store._history_parts(self._handles, lens)
+
+    def ids(self, parts: Sequence[torch.Tensor], offsets: torch.Tensor, total: int) -> torch.Tensor:
+        return self._store._gathered(parts, offsets, total)
+
+
+class HistoryStore(StoreSampling):
     """Append-only prior-token histories in one int32 device pool."""
 
     def __init__(self, device, capacity: int, vocab: int):
@@ -101,6 +184,7 @@ class HistoryStore:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._alloc = RegionAllocator(self.capacity)
         self._regions: Dict[int, List[int]] = {}  # handle -> [start, length, reserved]
+        self._prompts: Dict[int, int] = {}  # handle -> ids of the prompt
         self._next = 0
         self._staging = _Staging()
         self._append_staging = _Staging()
@@ -123,14 +207,19 @@ class HistoryStore:
         h = self._next
         self._next += 1
         self._regions[h] = [start, int(ids.size), reserved]
+        self._prompts[h] = int(ids.size)
         return h
 
     def release(self, handle: int) -> None:
         start, _, reserved = self._regions.pop(handle)
+        del self._prompts[handle]
         self._alloc.free(start, reserved)
 
     def length(self, handle: int) -> int:
         return self._regions[handle][1]
+
+    def prompt_length(self, handle: int) -> int:
+        return self._prompts[handle]
 
     def tokens(self, handle: int) -> List[int]:
         """The request's ids as a list (synchronises; for tests and debugging)."""
@@ -178,6 +267,14 @@ class HistoryStore:
                                 ids.data_ptr(), self.status.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
         return row_params, off_d, ids, order_d
 
+    def _history_parts(self, handles: Sequence[int], lens: np.ndarray) -> List[np.ndarray]:
+        return [np.fromiter((self._regions[h][0] for h in handles), dtype=np.int64, count=len(handles))]
+
+    def _history_ids(self, parts: Sequence[torch.Tensor], offsets: torch.Tensor, ids: torch.Tensor) -> None:
+        _cabi.ns_history_gather(self.pool.data_ptr(), self.capacity, parts[0].data_ptr(), offsets.data_ptr(),
+                                parts[0].numel(), ids.data_ptr(), self.status.data_ptr(),
+                                torch.cuda.current_stream(self.device).cuda_stream)
+
     def append(self, handles: Sequence[int], tokens: torch.Tensor) -> None:
         """Append ``tokens[i]`` (device int64 or int32 [S]) to request ``handles[i]``."""
         S = len(handles)
@@ -202,20 +299,3 @@ class HistoryStore:
                                 self.status.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
         for r in reg:
             r[1] += 1
-
-    def sample(self, sampler: Sampler, logits: torch.Tensor, sampling_params_list: Sequence, handles: Sequence[int],
-               *, append: bool = True, **kw):
-        """``Sampler.sample`` with the histories taken from this store; the
-        sampled ids are appended to the requests' histories (``append``).
-        Runs on the store's device (whatever device is current) inside an NVTX
-        range named ``logits+sample`` (nanoserve/engine/engine.py:234)."""
-        torch.cuda.nvtx.range_push("logits+sample")
-        try:
-            with torch.cuda.device(self.device):
-                rp, off, ids, order = self.pack(sampling_params_list, handles, sms=_sm_count(logits.device))
-                out = sampler.sample_packed(logits, rp, off, ids, row_order=order, **kw)
-                if append:
-                    self.append(handles, out[0] if isinstance(out, tuple) else out)
-                return out
-        finally:
-            torch.cuda.nvtx.range_pop()

@@ -19,6 +19,10 @@ ignores) gets its own Philox key and, as the counter, the length of its
 history (prompt plus tokens so far): the same request in the same state
 draws the same number whatever batch it is in.
 
+Requests may also carry ``presence_penalty``, ``frequency_penalty`` and
+``logit_bias`` (``ExtendedSamplingParams``): ``pack_processing`` turns them,
+and the repetition penalty, into the arrays of ``NsProcessArgs``.
+
 It also builds the optional row order (``NsSampleArgs.row_order``), a
 scheduling hint that starts the rows with the longest finishing work first.
 """
@@ -199,3 +203,69 @@ def to_bytes(packed: Packed, out: Optional[np.ndarray] = None) -> np.ndarray:
     if packed.order is not None:
         out[d : d + packed.order.nbytes] = packed.order.view(np.uint8)
     return out
+
+
+EXTENDED_FIELDS = ("presence_penalty", "frequency_penalty", "logit_bias")
+
+
+def wants_processing(params: Sequence) -> bool:
+    """Whether some request carries a presence or frequency penalty or a bias.
+    Looks at the requests only if one of their types has these fields."""
+    types = {type(p): p for p in params}
+    if not any(hasattr(p, f) for p in types.values() for f in EXTENDED_FIELDS):
+        return False
+    return any(getattr(p, f, None) for p in params for f in EXTENDED_FIELDS)
+
+
+@dataclass
+class Processing:
+    """One step's rows for ``process_logits`` (host arrays; history ids apart)."""
+
+    lens: np.ndarray          # int64 [S]    ids of each row's history that are needed (0: none)
+    offsets: np.ndarray       # int64 [S+1]  their CSR offsets
+    prompt_lens: np.ndarray   # int32 [S]
+    repetition: np.ndarray    # float32 [S]
+    presence: np.ndarray      # float32 [S]
+    frequency: np.ndarray     # float32 [S]
+    bias_offsets: np.ndarray  # int64 [S+1]
+    bias_ids: np.ndarray      # int32 [B]
+    bias_values: np.ndarray   # float32 [B]
+
+
+def pack_processing(params: Sequence, hist_lens, prompt_lens: Optional[Sequence[int]], vocab: int) -> Processing:
+    """The arrays of one step.  ``prompt_lens[i]`` ids of row i's history are its
+    prompt (None: no row has one, every id counts as generated).  A bias for a
+    token outside ``[0, vocab)`` raises ``IndexError``."""
+    S = len(params)
+    hist = np.asarray(hist_lens, dtype=np.int64)
+    prompt = np.zeros(S, dtype=np.int64) if prompt_lens is None else np.asarray(prompt_lens, dtype=np.int64)
+    if prompt.shape != (S,):
+        raise ValueError(f"{prompt.size} prompt lengths for {S} sampling params")
+    rep = np.array([p.repetition_penalty for p in params], dtype=np.float64).astype(np.float32)
+    pres = np.array([getattr(p, "presence_penalty", 0.0) or 0.0 for p in params], dtype=np.float64).astype(np.float32)
+    freq = np.array([getattr(p, "frequency_penalty", 0.0) or 0.0 for p in params], dtype=np.float64).astype(np.float32)
+    lens = np.where((rep != 1.0) | (pres != 0.0) | (freq != 0.0), hist, 0)
+    offsets = np.zeros(S + 1, dtype=np.int64)
+    np.cumsum(lens, out=offsets[1:])
+    biases = [getattr(p, "logit_bias", None) or {} for p in params]
+    bias_offsets = np.zeros(S + 1, dtype=np.int64)
+    np.cumsum([len(b) for b in biases], out=bias_offsets[1:])
+    total = int(bias_offsets[-1])
+    ids = np.fromiter((int(t) for b in biases for t in b), dtype=np.int64, count=total)
+    values = np.fromiter((float(v) for b in biases for v in b.values()), dtype=np.float64, count=total)
+    if total and (int(ids.min()) < 0 or int(ids.max()) >= vocab):
+        bad = int(ids.min()) if int(ids.min()) < 0 else int(ids.max())
+        raise IndexError(f"logit_bias token id {bad} is out of range for vocab size {vocab}")
+    return Processing(lens, offsets, np.clip(prompt, 0, 0x7FFFFFFF).astype(np.int32), rep, pres, freq, bias_offsets,
+                      ids.astype(np.int32), values.astype(np.float32))
+
+
+def flatten_histories(histories: Sequence[Sequence[int]], lens: np.ndarray, vocab: int) -> np.ndarray:
+    """The ids (int32) of the rows with ``lens[i] > 0``, one after the other, checked against ``vocab``."""
+    rows = np.flatnonzero(lens)
+    total = int(lens.sum())
+    ids = np.fromiter(itertools.chain.from_iterable(histories[i] for i in rows), dtype=np.int64, count=total)
+    if total and (int(ids.min()) < 0 or int(ids.max()) >= vocab):
+        bad = int(ids.min()) if int(ids.min()) < 0 else int(ids.max())
+        raise IndexError(f"history token id {bad} is out of range for vocab size {vocab}")
+    return ids.astype(np.int32)

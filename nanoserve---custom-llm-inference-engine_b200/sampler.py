@@ -22,6 +22,10 @@ Differences from the reference, all additive:
   the reference ignores, gives a request its own stream, keyed by the seed
   and the length of its history, so it draws the same tokens whatever batch
   it is in;
+* requests may carry presence and frequency penalties and a ``logit_bias``
+  (``ExtendedSamplingParams``), and ``allowed`` masks the tokens that a grammar
+  allows; ``logprobs=n`` also returns the log-probabilities of the sampled
+  tokens and of the ``n`` most likely ones;
 * ``generators`` is accepted and ignored, as in the reference (sampler.py:26);
 * ``sample_async`` returns int32 ids through a non-blocking copy to pinned
   host memory (``PendingTokens.wait()``), in place of the caller's blocking
@@ -156,6 +160,8 @@ class Sampler:
         call first waits for the oldest."""
         if kw.get("return_debug"):
             raise ValueError("sample_async returns ids only; use sample(return_debug=True) for debug outputs")
+        if kw.get("logprobs") is not None:
+            raise ValueError("sample_async returns ids only; use sample(logprobs=n) for log-probabilities")
         kw["out_dtype"] = torch.int32
         out = self.sample(logits, sampling_params_list, history_token_ids, generators, **kw)
         return self._ring.copy(out)
@@ -178,11 +184,27 @@ class Sampler:
         seed: Optional[int] = None,
         out_dtype: torch.dtype = torch.int64,
         return_debug: bool = False,
+        prompt_lens: Optional[Sequence[int]] = None,
+        allowed: Optional[torch.Tensor] = None,
+        allowed_rows: Optional[torch.Tensor] = None,
+        logprobs: Optional[int] = None,
     ):
+        """The next token of every row.
+
+        Rows whose parameters carry presence or frequency penalties or a
+        ``logit_bias`` (``ExtendedSamplingParams``), or any row when ``allowed`` is
+        given, are first processed by :func:`process_logits` (into a copy;
+        ``prompt_lens[i]`` ids of row i's history are its prompt, ``allowed`` and
+        ``allowed_rows`` are that function's device tensors).  With ``logprobs=n``
+        the result is ``(result, TokenLogprobs)``: the log-probabilities, over the
+        processed logits before temperature and filters, of the sampled tokens
+        and of the ``n`` most likely ones."""
         if logits.dim() != 2:
             raise ValueError("logits must be [num_seqs, vocab]")
         if not logits.is_cuda:
             raise RuntimeError("Sampler.sample needs CUDA logits (no CPU fallback)")
+        if allowed_rows is not None and allowed is None:
+            raise ValueError("allowed_rows given without allowed")
         vocab = logits.shape[1]
         S = len(sampling_params_list)
         if sample_indices is None and logits.shape[0] != S:
@@ -192,16 +214,70 @@ class Sampler:
             # every copy, event and launch below goes to the logits' device,
             # whatever device is current for the caller
             with torch.cuda.device(logits.device):
+                step = dict(uniforms=uniforms, seed=seed, out_dtype=out_dtype, return_debug=return_debug)
+                if allowed is not None or packing.wants_processing(sampling_params_list):
+                    return self._sample_processed(
+                        logits, sampling_params_list, _ListHistories(history_token_ids, S, vocab), prompt_lens,
+                        sample_indices=sample_indices, allowed=allowed, allowed_rows=allowed_rows, logprobs=logprobs,
+                        **step,
+                    )
                 packed = packing.pack(sampling_params_list, history_token_ids, vocab,
                                       sms=_sm_count(logits.device))
                 row_params, offsets, ids, order = self._upload(packed, logits.device)
-                return self.sample_packed(
-                    logits, row_params, offsets, ids,
-                    sample_indices=sample_indices, uniforms=uniforms, seed=seed,
-                    out_dtype=out_dtype, return_debug=return_debug, row_order=order,
+                out = self.sample_packed(
+                    logits, row_params, offsets, ids, sample_indices=sample_indices, row_order=order, **step,
                 )
+                return self._with_logprobs(out, logits, logprobs, sample_indices)
         finally:
             torch.cuda.nvtx.range_pop()
+
+    def _sample_processed(self, logits: torch.Tensor, params: Sequence, histories, prompt_lens, *,
+                          sample_indices: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                          allowed_rows: Optional[torch.Tensor] = None, logprobs: Optional[int] = None, **step):
+        """``sample`` with the logits processed first (penalties, the
+        repetition penalty among them, biases and masks), into an fp32 copy of
+        the sampled rows.  ``histories`` gives the lengths of the rows'
+        histories, the host arrays to upload for the ids of the rows that need
+        them, and those ids on the device."""
+        from .logits import process_logits
+
+        dev, vocab = logits.device, logits.shape[1]
+        if sample_indices is None and logits.shape[0] != len(params):
+            raise ValueError(f"logits has {logits.shape[0]} rows but {len(params)} sampling params were given")
+        lens = histories.lens()
+        pr = packing.pack_processing(params, lens, prompt_lens, vocab)
+        rows = packing.derive_rows(params, vocab, lens)
+        rows["flags"] &= ~np.uint32(packing._cabi.NS_ROW_PENALTY)  # applied here
+        order = packing.schedule(rows, _sm_count(dev))
+        # what no row uses is neither uploaded nor applied
+        total = int(pr.offsets[-1])
+        parts = {"rows": rows.view(np.uint8), "order": order}
+        if total:
+            parts.update(history_offsets=pr.offsets, repetition_penalty=pr.repetition,
+                         presence_penalty=pr.presence, frequency_penalty=pr.frequency)
+            if prompt_lens is not None:
+                parts["prompt_lens"] = pr.prompt_lens
+        if pr.bias_ids.size:
+            parts.update(bias_offsets=pr.bias_offsets, bias_ids=pr.bias_ids, bias_values=pr.bias_values)
+        more = histories.parts(pr.lens) if total else []
+        up = upload_parts(self._staging, [*parts.values(), *more], dev)
+        given = dict(zip(parts, up))
+        row_params, order_d = given.pop("rows"), given.pop("order")
+        if total:
+            given["history_ids"] = histories.ids(up[len(parts):], given["history_offsets"], total)
+        processed = process_logits(logits.detach(), sample_indices=sample_indices, allowed=allowed,
+                                   allowed_rows=allowed_rows, out_dtype=torch.float32, **given)
+        out = self.sample_packed(processed, row_params, None, None, row_order=order_d, **step)
+        return self._with_logprobs(out, processed, logprobs, None)
+
+    @staticmethod
+    def _with_logprobs(out, logits: torch.Tensor, logprobs: Optional[int], sample_indices: Optional[torch.Tensor]):
+        if logprobs is None:
+            return out
+        from .logprobs import token_logprobs
+
+        tokens = out[0] if isinstance(out, tuple) else out
+        return out, token_logprobs(logits.detach(), tokens, logprobs, sample_indices=sample_indices)
 
     # -- pre-packed device inputs (graph-capturable) ------------------------
     def sample_packed(
@@ -270,6 +346,45 @@ class Sampler:
             offsets = None
         order = dev[d : d + packed.order.nbytes].view(torch.int32) if packed.order is not None else None
         return row_params, offsets, ids, order
+
+
+class _ListHistories:
+    """Histories given as Python lists, for ``_sample_processed``."""
+
+    def __init__(self, histories: Sequence[Sequence[int]], rows: int, vocab: int):
+        if len(histories) < rows:
+            raise IndexError("history_token_ids has fewer entries than sampling_params_list")
+        self._histories, self._rows, self._vocab = histories, rows, vocab
+
+    def lens(self) -> np.ndarray:
+        return np.fromiter((len(self._histories[i]) for i in range(self._rows)), dtype=np.int64, count=self._rows)
+
+    def parts(self, lens: np.ndarray) -> List[np.ndarray]:
+        return [packing.flatten_histories(self._histories, lens, self._vocab)]
+
+    def ids(self, parts: Sequence[torch.Tensor], offsets: torch.Tensor, total: int) -> torch.Tensor:
+        return parts[0]
+
+
+_TORCH_DTYPES = {np.dtype(np.uint8): torch.uint8, np.dtype(np.int32): torch.int32, np.dtype(np.int64): torch.int64,
+                 np.dtype(np.float32): torch.float32}
+
+
+def upload_parts(staging: _Staging, arrays: Sequence[np.ndarray], device: torch.device) -> List[torch.Tensor]:
+    """The arrays on ``device`` (the current one), through one pinned buffer and one copy on the current stream."""
+    at, end = [], 0
+    for a in arrays:
+        at.append(end)
+        end = (end + a.nbytes + 15) & ~15
+    host = staging.get(max(end, 16))
+    hb = host.numpy()
+    for a, o in zip(arrays, at):
+        hb[o : o + a.nbytes] = np.ascontiguousarray(a).view(np.uint8).reshape(-1)
+    dev = host.to(device, non_blocking=True)
+    ev = torch.cuda.Event()
+    ev.record(torch.cuda.current_stream(device))
+    staging.event = ev
+    return [dev[o : o + a.nbytes].view(_TORCH_DTYPES[a.dtype]) for a, o in zip(arrays, at)]
 
 
 def upload_packed(packed: packing.Packed, device) -> tuple:
