@@ -11,10 +11,10 @@
 // (its bucket).  A thread keeps its bucket's maximum, its sum of exponentials
 // over a reference that follows the maximum in steps, and its count of larger
 // logits.  The n largest are then in few buckets: those whose maximum reaches
-// a bound that n buckets are known to reach.  Only these are read again (out of
-// L2), into a sorted list of 32 per warp, and the lists are merged, within the
-// block through shared memory and within the cluster through distributed
-// shared memory.
+// the n-th largest bucket maximum.  Only these are read again (out of L2); the
+// elements that reach the bound are ranked by counting (or, where ties make
+// them many, through sorted lists), within the block and then, through
+// distributed shared memory, within the cluster.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -34,7 +34,9 @@ constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
 constexpr int kMaxCluster = 8;     // the portable limit
 constexpr float kLag = 8.0f;       // the reference follows the maximum in steps of at least this
 constexpr float kHuge = 0x1p100f;  // beyond it the fused argument of the exponential could overflow
+constexpr int kCands = 256;        // candidates that are ranked by counting
 typedef unsigned long long u64;
+static_assert(kMaxCluster * NS_MAX_TOP_LOGPROBS <= kThreads, "the cluster's lists fit into s_list");
 
 // Larger value first, then smaller id, as one key to maximise; -0 counts as 0.
 // No logit's key is 0.
@@ -177,18 +179,6 @@ __device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
   return c;
 }
 
-__device__ __forceinline__ u64 sort_descending(u64 k, int lane) {
-#pragma unroll
-  for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll
-    for (int o = n >> 1; o; o >>= 1) {
-      const u64 p = __shfl_xor_sync(0xffffffffu, k, o);
-      const bool keep_max = ((lane & n) == 0) == ((lane & o) == 0);
-      k = keep_max == (p > k) ? p : k;
-    }
-  return k;
-}
-
 // Puts key c (the same in every lane) into the list.
 __device__ __forceinline__ u64 insert(u64 list, u64 c, int lane) {
   const int at = __popc(__ballot_sync(0xffffffffu, list > c));
@@ -210,8 +200,10 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   __shared__ float s_max[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_cnt[kWarps];
-  __shared__ uint32_t s_few[kWarps], s_all[kWarps];
-  __shared__ u64 s_list[kWarps > kMaxCluster ? kWarps : kMaxCluster][32];
+  __shared__ uint32_t s_few[kWarps], s_bound;
+  __shared__ int s_buckets, s_cands;
+  __shared__ u64 s_list[kThreads];  // buckets, then sorted keys
+  __shared__ u64 s_cand[kCands];
   __shared__ Part s_part[kMaxCluster];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int row = blockIdx.x / C, rank = blockIdx.x % C;
@@ -276,19 +268,20 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
     if (y > -INFINITY) sum.s += exp_shifted(y, sum.ref) * ex2_approx(sum.lo);
   }
 
-  // block maximum, counts, and the bound on bucket maxima
+  // block maximum and count
   float bm = m;
 #pragma unroll
   for (int o = 16; o; o >>= 1) bm = fmax_nan(bm, __shfl_xor_sync(0xffffffffu, bm, o));
   cnt = __reduce_add_sync(0xffffffffu, cnt);
-  u64 order = 0;  // the warp's buckets, the largest maximum first: (maximum, 31 - lane)
   if (n > 0) {
-    order = sort_descending(((u64)bucket << 32) | (uint32_t)(31 - lane), lane);
-    // Each warp has (n + kWarps - 1) / kWarps buckets that reach its `few`, so
-    // n buckets reach the least of these; and n buckets reach the largest `all`.
-    const uint32_t few = __shfl_sync(0xffffffffu, (uint32_t)(order >> 32), (n + kWarps - 1) / kWarps - 1);
-    const uint32_t all = __shfl_sync(0xffffffffu, (uint32_t)(order >> 32), n - 1);
-    if (lane == 0) s_few[warp] = few, s_all[warp] = all;
+    // the q-th largest bucket maximum of the warp, q = ceil(n / kWarps)
+    uint32_t left = bucket, few = 0;
+    for (int q = 0; q < n; q += kWarps) {
+      few = __reduce_max_sync(0xffffffffu, left);
+      if (__ffs(__ballot_sync(0xffffffffu, left == few)) - 1 == lane) left = 0;
+    }
+    if (lane == 0) s_few[warp] = few;
+    if (tid == 0) s_buckets = s_cands = 0;
   }
   if (lane == 0) s_max[warp] = bm, s_cnt[warp] = cnt;
   __syncthreads();
@@ -299,46 +292,117 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   if (lane == 0) s_sum[warp] = part;
 
   if (n > 0) {
-    uint32_t few = s_few[0], bound = s_all[0];
+    // n buckets reach the least of the warps' q-th maxima: list the buckets that do, and find the
+    // n-th largest maximum (0 if there are fewer) among them
+    uint32_t few = s_few[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) few = min(few, s_few[w]), bound = max(bound, s_all[w]);
-    bound = max(bound, few);
-    u64 list = 0;
-    for (uint32_t take = __ballot_sync(0xffffffffu, odd_key != 0); take; take &= take - 1)
-      list = insert(list, __shfl_sync(0xffffffffu, odd_key, __ffs(take) - 1), lane);
-    for (int k = 0; k < 32; ++k) {
-      const u64 o = __shfl_sync(0xffffffffu, order, k);
-      const uint32_t best = (uint32_t)(o >> 32);
-      if (best == 0 || best < bound) break;
-      const int first = lo + warp * 32 + 31 - (int)(uint32_t)o;  // the bucket's first vector
-      u64 nth = __shfl_sync(0xffffffffu, list, n - 1);
-      if ((((u64)best << 32) | (uint32_t)~(head + first * kVec)) <= nth) continue;
-      for (int j = first; j < hi; j += 32 * kThreads) {
-        const int mine = j + lane * kThreads;
-        Vec b;
-        if (mine < hi) b.load(xv + (int64_t)mine * kVec);
+    for (int w = 1; w < kWarps; ++w) few = n == 1 ? max(few, s_few[w]) : min(few, s_few[w]);
+    if (bucket && bucket >= few) s_list[atomicAdd(&s_buckets, 1)] = ((u64)bucket << 32) | (uint32_t)tid;
+    if (tid == 0) s_bound = few;
+    __syncthreads();
+    const int nb = s_buckets;
+    if (n > 1 && tid < nb) {
+      const uint32_t mine = (uint32_t)(s_list[tid] >> 32);
+      int more = 0, same = 0;
+      for (int j = 0; j < nb; ++j) {
+        const uint32_t k = (uint32_t)(s_list[j] >> 32);
+        more += k > mine, same += k == mine;
+      }
+      if (more < n && n <= more + same) s_bound = mine;  // one value, whoever writes it
+    }
+    __syncthreads();
+    // every element that reaches the bound is in one of these buckets: read them again
+    const u64 bound = (u64)s_bound << 32;
+    const int chunks = (hi - lo + 32 * kThreads - 1) / (32 * kThreads);
+    const int items = nb * chunks;
+    for (int k = warp; k < items; k += kWarps * kUnroll) {
+      Vec b[kUnroll];
+      int at[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int item = k + u * kWarps;
+        at[u] = -1;
+        if (item < items) {
+          const u64 e = s_list[item / chunks];
+          const int j = lo + (int)(uint32_t)e + ((item % chunks) * 32 + lane) * kThreads;
+          if (e >= bound && j < hi) at[u] = j;
+        }
+        if (at[u] >= 0) b[u].load(xv + (int64_t)at[u] * kVec);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (at[u] < 0) continue;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const u64 key = mine < hi ? top_key(b.get(e), head + mine * kVec + e) : 0;
-          for (uint32_t take = __ballot_sync(0xffffffffu, key > nth); take; take &= take - 1) {
-            const u64 c = __shfl_sync(0xffffffffu, key, __ffs(take) - 1);
-            if (c > nth) {
-              list = insert(list, c, lane);
-              nth = __shfl_sync(0xffffffffu, list, n - 1);
-            }
+          const u64 key = top_key(b[u].get(e), head + at[u] * kVec + e);
+          if (key >= bound) {
+            const int c = atomicAdd(&s_cands, 1);
+            if (c < kCands) s_cand[c] = key;
           }
         }
       }
     }
-    s_list[warp][lane] = list;
-#pragma unroll
-    for (int s = 1; s < kWarps; s <<= 1) {
-      __syncthreads();
-      if (warp % (2 * s) == 0) {
-        list = merge_lists(list, s_list[warp + s][lane], lane);
-        s_list[warp][lane] = list;
-      }
+    if (odd_key >= bound && odd_key) {
+      const int c = atomicAdd(&s_cands, 1);
+      if (c < kCands) s_cand[c] = odd_key;
     }
+    __syncthreads();
+    const int nc = s_cands;
+    u64 mine = 0;
+    int place = 32;
+    if (nc <= kCands) {
+      // few candidates: each counts the larger ones
+      if (tid < nc) {
+        mine = s_cand[tid];
+        place = 0;
+        for (int j = 0; j < nc; ++j) place += s_cand[j] > mine;
+      }
+    } else {
+      // many equal or close ones: sorted lists, one per warp, merged.  A bucket whose best possible key
+      // cannot enter its warp's list is not read.
+      u64 list = 0;
+      for (uint32_t take = __ballot_sync(0xffffffffu, odd_key != 0); take; take &= take - 1)
+        list = insert(list, __shfl_sync(0xffffffffu, odd_key, __ffs(take) - 1), lane);
+      for (int k = warp; k < nb; k += kWarps) {
+        const u64 e = s_list[k];
+        if (e < bound) continue;
+        const int first = lo + (int)(uint32_t)e;  // the bucket's first vector
+        u64 nth = __shfl_sync(0xffffffffu, list, n - 1);
+        if (((e >> 32 << 32) | (uint32_t)~(head + first * kVec)) <= nth) continue;
+        for (int j = first; j < hi; j += 32 * kThreads) {
+          const int at = j + lane * kThreads;
+          Vec b;
+          if (at < hi) b.load(xv + (int64_t)at * kVec);
+#pragma unroll
+          for (int q = 0; q < kVec; ++q) {
+            const u64 key = at < hi ? top_key(b.get(q), head + at * kVec + q) : 0;
+            for (uint32_t take = __ballot_sync(0xffffffffu, key > nth); take; take &= take - 1) {
+              const u64 c = __shfl_sync(0xffffffffu, key, __ffs(take) - 1);
+              if (c > nth) {
+                list = insert(list, c, lane);
+                nth = __shfl_sync(0xffffffffu, list, n - 1);
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();  // the buckets have been read
+      s_list[tid] = list;
+#pragma unroll
+      for (int s = 1; s < kWarps; s <<= 1) {
+        __syncthreads();
+        if (warp % (2 * s) == 0) {
+          list = merge_lists(list, s_list[(warp + s) * 32 + lane], lane);
+          s_list[tid] = list;
+        }
+      }
+      if (warp == 0) mine = list, place = lane;
+    }
+    // the block's best n, in order; a slice with fewer elements leaves zeros
+    __syncthreads();
+    if (tid < 32) s_list[tid] = 0;
+    __syncthreads();
+    if (place < n) s_list[place] = mine;
   }
   __syncthreads();
   Part p;
@@ -346,12 +410,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   if (warp == 0) {
     for (int w = 0; w < kWarps; ++w) p.sum += s_sum[w];
   }
-  u64 list = n > 0 ? s_list[0][lane] : 0;  // warp 0's own
   if (C > 1) {
     // every block's part and list to the first block of the cluster
-    if (rank != 0) cluster_arrive_relaxed();
-    else cluster_arrive();
-    cluster_wait();  // every block of the cluster runs and is done with its lists
+    cluster_sync();  // every block of the cluster runs and is done with its lists
     if (warp == 0 && rank != 0) {
       const uint32_t to = dsmem_map(smem_addr(&s_part[rank]), 0);
       if (lane == 0) {
@@ -359,21 +420,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
         dsmem_st_f32(to + offsetof(Part, max), p.max);
         dsmem_st_u32(to + offsetof(Part, count), (uint32_t)p.count);
       }
-      if (n > 0) dsmem_st_u64(dsmem_map(smem_addr(&s_list[rank][lane]), 0), list);
+      if (lane < n) dsmem_st_u64(dsmem_map(smem_addr(&s_list[rank * n + lane]), 0), s_list[lane]);
     }
     cluster_sync();
     if (rank != 0) return;
-    if (n > 0)
-      for (int s = 1; s < C; s <<= 1) {
-        if (warp % (2 * s) == 0 && warp + s < C) {
-          list = merge_lists(s_list[warp][lane], s_list[warp + s][lane], lane);
-          s_list[warp][lane] = list;
-        }
-        __syncthreads();
-      }
+    if (n > 0) {
+      // each of the blocks' best counts the larger ones
+      const u64 mine = tid < C * n ? s_list[tid] : 0;
+      int place = 0;
+      for (int j = 0; j < C * n; ++j) place += s_list[j] > mine;
+      __syncthreads();
+      if (mine && place < n) s_list[place] = mine;
+      __syncthreads();
+    }
   }
   if (warp != 0) return;
-  if (n > 0) list = s_list[0][lane];
+  const u64 list = lane < n ? s_list[lane] : 0;
   float top = p.max;
   for (int c = 1; c < C; ++c) top = fmax_nan(top, s_part[c].max), p.count += s_part[c].count;
   const bool uniform = !(fabsf(top) < INFINITY);  // NaN, +inf, or only -inf
