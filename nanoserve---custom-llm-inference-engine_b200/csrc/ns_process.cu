@@ -7,15 +7,16 @@
 //   x = x + bias             where the row has one
 //   x = -inf                 where the row's mask bit is 0
 //
-// A block owns one tile of kTile vocabulary ids of one row.  It counts the
-// row's history ids that fall into its tile in shared memory (one 32-bit word
-// per id: the count, a bit for the prompt, bits for biases), copies the tile
-// through (masked), and then recomputes the few ids that a penalty or a bias
-// names from the input.
+// Two kernels.  tile_kernel writes whole rows (or, in place, what a mask
+// forbids): a block owns a tile of kTile vocabulary ids of one row.
+// sparse_kernel serves calls in place without masks, which change only the ids
+// that a history or a bias names: a block owns a row (or a part of its ids).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <mutex>
 #include <string>
 
 #include "ns_device.cuh"
@@ -27,6 +28,8 @@ namespace proc {
 
 constexpr int kThreads = 256;
 constexpr int kTile = 8192;  // multiple of 32: a tile starts on a mask word
+constexpr int kHits = 2048;
+constexpr uint32_t kMaxTries = 1u << 22;
 
 // Word of one vocabulary id: occurrences after the prompt in the low bits.
 constexpr uint32_t kInPrompt = 1u << 31;
@@ -35,25 +38,18 @@ constexpr uint32_t kBiasTwice = 1u << 29;
 constexpr uint32_t kCount = kBiasTwice - 1;
 constexpr int64_t kMaxRowIds = 1 << 28;  // a row's counts fit below the flag bits
 
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p);
-template <>
-__device__ __forceinline__ float load_f<float>(const float* p) {
-  return *p;
-}
-template <>
-__device__ __forceinline__ float load_f<__nv_bfloat16>(const __nv_bfloat16* p) {
-  return __bfloat162float(*p);
-}
+__device__ __forceinline__ float load_f(const float* p) { return *p; }
+__device__ __forceinline__ float load_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void store_f(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_f(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // [o[row], o[row+1]) of an array of `total` entries; empty (and flagged) where
 // it leaves the array or is too long to count.
 __device__ __forceinline__ int row_range(const int64_t* o, int row, int64_t total, int64_t* first, uint32_t* bad) {
-  const int64_t a = o[row], b = o[row + 1];
+  const int64_t a = __ldg(o + row), b = __ldg(o + row + 1);
   *first = a;
   if (a >= 0 && b >= a && b <= total && b - a <= kMaxRowIds) return (int)(b - a);
+  *first = 0;
   *bad |= NS_STATUS_BAD_ROW_RANGE;
   return 0;
 }
@@ -69,9 +65,89 @@ __device__ __forceinline__ float penalised(float x, uint32_t w, const Penalty& p
   return x;
 }
 
+// What one row asks for.
+struct RowWork {
+  Penalty pen;
+  const int32_t *hist, *bias;
+  const float* value;
+  int hn, bn, prompt;
+  uint32_t bad;
+};
+
+__device__ __forceinline__ RowWork row_work(const NsProcessArgs& a, int row) {
+  RowWork r;
+  r.bad = 0;
+  r.pen.rep = a.repetition_penalty ? __ldg(a.repetition_penalty + row) : 1.0f;
+  r.pen.pres = a.presence_penalty ? __ldg(a.presence_penalty + row) : 0.0f;
+  r.pen.freq = a.frequency_penalty ? __ldg(a.frequency_penalty + row) : 0.0f;
+  int64_t h0 = 0, b0 = 0;
+  r.hn = a.history_offsets ? row_range(a.history_offsets, row, a.num_history_ids, &h0, &r.bad) : 0;
+  r.bn = a.bias_offsets ? row_range(a.bias_offsets, row, a.num_biases, &b0, &r.bad) : 0;
+  r.prompt = a.prompt_lens ? __ldg(a.prompt_lens + row) : 0;
+  if (r.pen.rep == 1.0f && r.pen.pres == 0.0f && r.pen.freq == 0.0f) r.hn = 0;  // nothing would change
+  r.hist = a.history_ids + h0;
+  r.bias = a.bias_ids + b0;
+  r.value = a.bias_values + b0;
+  return r;
+}
+
+// f(j, id of entry j) for all n ids, kThreads apart, four loads in flight.
+template <int kBlock, typename F>
+__device__ __forceinline__ void for_ids(const int32_t* ids, int n, F f) {
+  for (int j = threadIdx.x; j < n; j += 4 * kBlock) {
+    int v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = j + u * kBlock < n ? __ldg(ids + j + u * kBlock) : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (j + u * kBlock < n) f(j + u * kBlock, v[u]);
+  }
+}
+
+// Entry j is the row's last for its id (asked only where an id has several).
+__device__ __forceinline__ bool last_entry(const RowWork& r, int j, int v) {
+  for (int k = j + 1; k < r.bn; ++k)
+    if (__ldg(r.bias + k) == v) return false;
+  return true;
+}
+
+// Bits [i, i + 32) of a mask of `words` words; those behind its end are 1.
+__device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int words, int i) {
+  const int w = i >> 5;
+  const uint32_t a = w < words ? __ldg(mask + w) : ~0u, b = w + 1 < words ? __ldg(mask + w + 1) : ~0u;
+  return __funnelshift_r(a, b, i & 31);
+}
+
+// Bulk copy of `bytes` (multiple of 16, both addresses 16-byte aligned) from this
+// CTA's shared memory to global memory, and the wait until it has been read.
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;" ::"l"(dst),
+               "r"(smem_addr(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_s2g_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+__device__ __forceinline__ bool wait_for(uint64_t* bar) {
+  for (uint32_t i = 0; i < kMaxTries; ++i)
+    if (mbar_try_wait(bar, 0)) return true;
+  return false;
+}
+
+// One tile of one row.  The tile is brought into shared memory by a bulk copy
+// while the block counts the row's history ids that fall into it, one 32-bit
+// word per id in shared memory (the count, a bit for the prompt, bits for
+// biases), and lists the ids it meets first.  Then each listed id's logit is
+// recomputed where it lies, and the tile leaves through a bulk copy, or, under a
+// mask or with another type, through registers.
 template <typename In, typename Out, bool kInPlace>
-__global__ void __launch_bounds__(kThreads) process_kernel(const NsProcessArgs a, int tiles) {
-  __shared__ uint32_t words[kTile];
+__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles) {
+  constexpr bool kSame = sizeof(In) == sizeof(Out);
+  constexpr int kVec = 16 / sizeof(In);
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem);
+  uint16_t* hits = reinterpret_cast<uint16_t*>(smem + kTile * 4);
+  __shared__ uint64_t bar;
+  __shared__ int s_hits;
   const int tid = threadIdx.x;
   const int row = blockIdx.x / tiles;
   const int v0 = (blockIdx.x % tiles) * kTile;
@@ -80,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) process_kernel(const NsProcessArgs a
 
   int64_t src = row;
   if (a.sample_indices) {
-    src = a.sample_indices[row];
+    src = __ldg(a.sample_indices + row);
     if (src < 0 || src >= a.num_logit_rows) {
       bad |= NS_STATUS_BAD_SAMPLE_INDEX;
       src = 0;
@@ -88,86 +164,322 @@ __global__ void __launch_bounds__(kThreads) process_kernel(const NsProcessArgs a
   }
   const In* in = static_cast<const In*>(a.logits) + src * a.logits_row_stride + v0;
   Out* out = static_cast<Out*>(a.out) + (int64_t)row * a.out_row_stride + v0;
+  // the tile in shared memory, at the same offset to the 16-byte grid as in global memory
+  const int skew = (int)(reinterpret_cast<uintptr_t>(in) & 15);
+  In* x = reinterpret_cast<In*>(smem + kTile * 4 + kHits * 2 + skew);
+  const int head = min(n, (16 - skew) % 16 / (int)sizeof(In));  // elements before the first 16-byte boundary
+  const int body = (n - head) / kVec * kVec;
+  if (!kInPlace) {
+    if (tid == 0) {
+      mbar_init(&bar, 1);
+      fence_mbar_init();
+      mbar_arrive_expect_tx(&bar, body * sizeof(In));
+      if (body) bulk_g2s(x + head, in + head, body * sizeof(In), &bar);
+    }
+    if (tid < head) x[tid] = in[tid];
+    if (tid < n - head - body) x[head + body + tid] = in[head + body + tid];
+  }
 
+  const RowWork r = row_work(a, row);
+  bad |= r.bad;
   const uint32_t* mask = nullptr;
   if (a.allowed) {
-    const int m = a.allowed_rows ? a.allowed_rows[row] : row;
+    const int m = a.allowed_rows ? __ldg(a.allowed_rows + row) : row;
     if (m >= a.num_masks) bad |= NS_STATUS_BAD_MASK_ROW;
     else if (m >= 0) mask = reinterpret_cast<const uint32_t*>(a.allowed) + m * a.mask_stride + v0 / 32;
   }
+  const int mask_words = (n + 31) / 32;
+  const bool counted = r.hn || r.bn;  // the same in all threads
 
-  Penalty pen;
-  pen.rep = a.repetition_penalty ? a.repetition_penalty[row] : 1.0f;
-  pen.pres = a.presence_penalty ? a.presence_penalty[row] : 0.0f;
-  pen.freq = a.frequency_penalty ? a.frequency_penalty[row] : 0.0f;
-  const bool counts = a.history_offsets && !(pen.rep == 1.0f && pen.pres == 0.0f && pen.freq == 0.0f);
-  int64_t h0 = 0, b0 = 0;
-  const int hn = counts ? row_range(a.history_offsets, row, a.num_history_ids, &h0, &bad) : 0;
-  const int bn = a.bias_offsets ? row_range(a.bias_offsets, row, a.num_biases, &b0, &bad) : 0;
-  const int32_t* hist = a.history_ids + h0;
-  const int32_t* bias = a.bias_ids + b0;
-  const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
-
-  if (hn || bn) {
-    for (int i = tid; i < n; i += kThreads) words[i] = 0;
+  if (tid == 0) s_hits = 0;
+  if (counted) {
+    for (int i = tid * 4; i < n; i += kThreads * 4) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int j = tid; j < hn; j += kThreads) {
-      const int v = hist[j];
+    for_ids<kThreads>(r.hist, r.hn, [&](int j, int v) {
       if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_HISTORY_ID;
       const uint32_t i = (uint32_t)(v - v0);
       if (i < (uint32_t)n) {
-        if (j < prompt) atomicOr(&words[i], kInPrompt);
-        else atomicAdd(&words[i], 1u);
+        const uint32_t was = j < r.prompt ? atomicOr(&words[i], kInPrompt) : atomicAdd(&words[i], 1u);
+        if (!(was & (kInPrompt | kCount))) {
+          const int h = atomicAdd(&s_hits, 1);
+          if (h < kHits) hits[h] = (uint16_t)i;
+        }
       }
-    }
-    for (int j = tid; j < bn; j += kThreads) {
-      const int v = bias[j];
+    });
+    for_ids<kThreads>(r.bias, r.bn, [&](int, int v) {
       if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_TOKEN_ID;
       const uint32_t i = (uint32_t)(v - v0);
       if (i < (uint32_t)n && (atomicOr(&words[i], kBias) & kBias)) atomicOr(&words[i], kBiasTwice);
-    }
+    });
   }
-  if (!kInPlace || mask) {
-    for (int i = tid; i < n; i += kThreads) {
-      const bool ok = !mask || ((mask[i >> 5] >> (i & 31)) & 1u);
-      if (!ok) store_f(out + i, -INFINITY);
-      else if (!kInPlace) store_f(out + i, load_f(in + i));
-    }
+  __syncthreads();  // also: the barrier is initialised, the tile's ends are there
+  if (!kInPlace && !wait_for(&bar)) {
+    if (tid == 0 && a.status) atomicOr(a.status, NS_STATUS_WAIT_TIMEOUT);
+    wait_for(&bar);  // the copy may still land
+    return;
   }
-  if (hn || bn) {
-    __syncthreads();
-    // biased ids first: the row's last entry for an id takes its word
-    for (int j = tid; j < bn; j += kThreads) {
-      const uint32_t i = (uint32_t)(bias[j] - v0);
-      if (i >= (uint32_t)n) continue;
+
+  // The ids that a penalty or a bias names.  `put` is where their results go: into the tile, before it is
+  // written; or, where the tile keeps another type or is not there, to the output.
+  const auto fix = [&](auto get, auto put) {
+    const auto history = [&](int i) {
       const uint32_t w = words[i];
-      if (!(w & kBias)) continue;  // taken by the id's last entry
-      if (w & kBiasTwice) {
-        bool last = true;
-        for (int k = j + 1; k < bn && last; ++k) last = bias[k] != bias[j];
-        if (!last) continue;
-      }
-      words[i] = 0;
-      if (mask && !((mask[i >> 5] >> (i & 31)) & 1u)) continue;
-      store_f(out + i, __fadd_rn(penalised(load_f(in + i), w, pen), a.bias_values[b0 + j]));
+      if (w && !(w & kBias)) put(i, penalised(get(i), w, r.pen));
+    };
+    const int nh = s_hits;
+    if (nh <= kHits)
+      for (int h = tid; h < nh; h += kThreads) history(hits[h]);
+    else
+      for (int i = tid; i < n; i += kThreads) history(i);
+    for_ids<kThreads>(r.bias, r.bn, [&](int j, int v) {
+      const uint32_t i = (uint32_t)(v - v0);
+      if (i >= (uint32_t)n) return;
+      const uint32_t w = words[i];
+      if (!(w & kBiasTwice) || last_entry(r, j, v))
+        put((int)i, __fadd_rn(penalised(get((int)i), w, r.pen), __ldg(r.value + j)));
+    });
+  };
+  const auto allowed = [&](int i) { return !mask || ((__ldg(mask + (i >> 5)) >> (i & 31)) & 1u); };
+
+  if constexpr (kInPlace) {
+    if (mask)
+      for (int i = tid; i < n; i += kThreads)
+        if (!allowed(i)) store_f(out + i, -INFINITY);
+    if (counted)
+      fix([&](int i) { return load_f(in + i); },
+          [&](int i, float y) {
+            if (allowed(i)) store_f(out + i, y);
+          });
+  } else if constexpr (kSame) {
+    if (counted) {
+      fix([&](int i) { return load_f(x + i); }, [&](int i, float y) { store_f(x + i, y); });
+      fence_proxy_async_smem();
+      __syncthreads();
     }
-    __syncthreads();
-    for (int j = tid; j < hn; j += kThreads) {
-      const uint32_t i = (uint32_t)(hist[j] - v0);
-      if (i >= (uint32_t)n) continue;
-      const uint32_t w = atomicExch(&words[i], 0u);
-      if (!w) continue;  // another occurrence, or a bias, has done it
-      if (mask && !((mask[i >> 5] >> (i & 31)) & 1u)) continue;
-      store_f(out + i, penalised(load_f(in + i), w, pen));
+    const bool aligned = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    if (!aligned) {
+      for (int i = tid; i < n; i += kThreads) {
+        if (allowed(i)) out[i] = x[i];
+        else store_f(out + i, -INFINITY);
+      }
+    } else {
+      if (!mask) {
+        if (tid == 0 && body) bulk_s2g(out + head, x + head, body * sizeof(Out));
+      } else {
+        for (int i = head + tid * kVec; i < head + body; i += kThreads * kVec) {
+          const uint32_t bits = mask_bits(mask, mask_words, i);
+          uint4 y = *reinterpret_cast<const uint4*>(x + i);
+          uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(In) == 4) {
+              if (!((bits >> e) & 1u)) w[e] = 0xff800000u;
+            } else {
+              if (!((bits >> (2 * e)) & 1u)) w[e] = (w[e] & 0xffff0000u) | 0xff80u;
+              if (!((bits >> (2 * e + 1)) & 1u)) w[e] = (w[e] & 0xffffu) | 0xff800000u;
+            }
+          }
+          *reinterpret_cast<uint4*>(out + i) = y;
+        }
+      }
+      const int e = tid < head ? tid : tid - head < n - head - body ? body + tid : -1;  // the ends
+      if (e >= 0) {
+        if (allowed(e)) out[e] = x[e];
+        else store_f(out + e, -INFINITY);
+      }
+      if (!mask && tid == 0) bulk_s2g_wait();  // shared memory is read before the block ends
+    }
+  } else {
+    // bf16 in, fp32 out
+    for (int i = tid * 2; i < n; i += kThreads * 2) {
+      const bool two = i + 1 < n;
+      const float y0 = allowed(i) ? load_f(x + i) : -INFINITY;
+      const float y1 = two && allowed(i + 1) ? load_f(x + i + (two ? 1 : 0)) : -INFINITY;
+      store_f(out + i, y0);
+      if (two) store_f(out + i + 1, y1);
+    }
+    if (counted) {
+      __syncthreads();
+      fix([&](int i) { return load_f(x + i); },
+          [&](int i, float y) {
+            if (allowed(i)) store_f(out + i, y);
+          });
     }
   }
   if (bad && a.status) atomicOr(a.status, bad);
 }
 
+// In place and without masks only the ids that a history or a bias names
+// change.  Block `row` counts its row's ids in a hash table in shared memory (open
+// addressing, at most half full) and recomputes each once.  Rows with more ids
+// than the table takes are left to the kHelpers blocks behind: every one finds
+// these rows, and they share out their ranges of kRange ids, one word per id.
+constexpr int kSparseThreads = 512;
+constexpr int kSlots = 8192;  // power of two
+constexpr int kRange = 2 * kSlots;
+constexpr int kHelpers = 148;
+
+template <typename T>
+__global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_constant__ NsProcessArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem);  // kSlots words and kSlots ids, or kRange words
+  uint32_t* ids = words + kSlots;                       // id + 1, 0: free
+  __shared__ uint32_t s_long[kSparseThreads / 32];
+  __shared__ int s_rows[kSparseThreads];
+  const int tid = threadIdx.x, lane = tid % 32;
+  const uint32_t V = (uint32_t)a.vocab_size;
+  uint32_t bad = 0;
+
+  if ((int)blockIdx.x < a.num_rows) {
+    const int row = blockIdx.x;
+    const RowWork r = row_work(a, row);
+    bad |= r.bad;
+    if (r.hn + r.bn > kSlots / 2) return;  // a long row
+    T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_row_stride;
+    int slots = 256;
+    while (slots < 2 * (r.hn + r.bn)) slots *= 2;
+    for (int i = tid; i < slots; i += kSparseThreads) words[i] = ids[i] = 0;
+    __syncthreads();
+    const auto slot_of = [&](uint32_t v) {  // v's slot, taken if it has none
+      uint32_t s = (v * 2654435761u) >> 12;
+      for (;; ++s) {
+        s &= slots - 1;
+        const uint32_t was = atomicCAS(&ids[s], 0u, v + 1);  // ends: the table is at most half full
+        if (was == 0 || was == v + 1) return s;
+      }
+    };
+    for_ids<kSparseThreads>(r.hist, r.hn, [&](int j, int v) {
+      if ((uint32_t)v >= V) {
+        bad |= NS_STATUS_BAD_HISTORY_ID;
+        return;
+      }
+      const uint32_t s = slot_of(v);
+      if (j < r.prompt) atomicOr(&words[s], kInPrompt);
+      else atomicAdd(&words[s], 1u);
+    });
+    for_ids<kSparseThreads>(r.bias, r.bn, [&](int, int v) {
+      if ((uint32_t)v >= V) {
+        bad |= NS_STATUS_BAD_TOKEN_ID;
+        return;
+      }
+      const uint32_t s = slot_of(v);
+      if (atomicOr(&words[s], kBias) & kBias) atomicOr(&words[s], kBiasTwice);
+    });
+    __syncthreads();
+    for (int i = tid; i < slots; i += 4 * kSparseThreads) {
+      uint32_t v[4], w[4];
+      float y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = i + u * kSparseThreads;
+        v[u] = s < slots ? ids[s] : 0;
+        w[u] = v[u] ? words[s] : 0;
+        if (w[u] & kBias) v[u] = 0;
+        y[u] = v[u] ? load_f(out + v[u] - 1) : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (v[u]) store_f(out + v[u] - 1, penalised(y[u], w[u], r.pen));
+    }
+    for_ids<kSparseThreads>(r.bias, r.bn, [&](int j, int v) {
+      if ((uint32_t)v >= V) return;
+      const uint32_t w = words[slot_of(v)];
+      if (!(w & kBiasTwice) || last_entry(r, j, v))
+        store_f(out + v, __fadd_rn(penalised(load_f(out + v), w, r.pen), __ldg(r.value + j)));
+    });
+  } else {
+    const int ranges = (a.vocab_size + kRange - 1) / kRange;
+    int64_t item = 0;  // of all rows' ranges, in order
+    for (int base = 0; base < a.num_rows; base += kSparseThreads) {
+      bool is_long = false;
+      if (base + tid < a.num_rows) {
+        const RowWork r = row_work(a, base + tid);
+        is_long = r.hn + r.bn > kSlots / 2;
+      }
+      const uint32_t vote = __ballot_sync(0xffffffffu, is_long);
+      if (lane == 0) s_long[tid / 32] = vote;
+      if (!__syncthreads_or(is_long)) continue;
+      int before = __popc(vote & ((1u << lane) - 1)), rows = 0;
+      for (int w = 0; w < kSparseThreads / 32; ++w) {
+        if (w < tid / 32) before += __popc(s_long[w]);
+        rows += __popc(s_long[w]);
+      }
+      if (is_long) s_rows[before] = base + tid;
+      __syncthreads();
+      for (int k = 0; k < rows * ranges; ++k, ++item) {
+        if (item % kHelpers != (int)blockIdx.x - a.num_rows) continue;
+        const int row = s_rows[k / ranges], v0 = (k % ranges) * kRange;
+        const uint32_t n = min(kRange, a.vocab_size - v0);
+        const RowWork r = row_work(a, row);
+        bad |= r.bad;
+        T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_row_stride + v0;
+        for (int i = tid; i < kRange; i += kSparseThreads) words[i] = 0;
+        __syncthreads();
+        for_ids<kSparseThreads>(r.hist, r.hn, [&](int j, int v) {
+          if ((uint32_t)v >= V) bad |= NS_STATUS_BAD_HISTORY_ID;
+          const uint32_t i = (uint32_t)(v - v0);
+          if (i >= n) return;
+          if (j < r.prompt) atomicOr(&words[i], kInPrompt);
+          else atomicAdd(&words[i], 1u);
+        });
+        for_ids<kSparseThreads>(r.bias, r.bn, [&](int, int v) {
+          if ((uint32_t)v >= V) bad |= NS_STATUS_BAD_TOKEN_ID;
+          const uint32_t i = (uint32_t)(v - v0);
+          if (i < n && (atomicOr(&words[i], kBias) & kBias)) atomicOr(&words[i], kBiasTwice);
+        });
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += kSparseThreads) {
+          const uint32_t w = words[i];
+          if (w && !(w & kBias)) store_f(out + i, penalised(load_f(out + i), w, r.pen));
+        }
+        for_ids<kSparseThreads>(r.bias, r.bn, [&](int j, int v) {
+          const uint32_t i = (uint32_t)(v - v0);
+          if (i >= n) return;
+          const uint32_t w = words[i];
+          if (!(w & kBiasTwice) || last_entry(r, j, v))
+            store_f(out + i, __fadd_rn(penalised(load_f(out + i), w, r.pen), __ldg(r.value + j)));
+        });
+        __syncthreads();  // words may be cleared
+      }
+      __syncthreads();  // s_long and s_rows may be written
+    }
+  }
+  if (bad && a.status) atomicOr(a.status, bad);
+}
+
+// Dynamic shared memory above 48 KB has to be allowed once per device and kernel.
+template <auto kernel>
+cudaError_t allow_smem(int bytes) {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lk(mu);
+  if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
+}
+
 template <typename In, typename Out, bool kInPlace>
-cudaError_t launch(const NsProcessArgs& a, cudaStream_t st) {
+cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
   const int tiles = (a.vocab_size + kTile - 1) / kTile;
-  process_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, 0, st>>>(a, tiles);
+  const int bytes = kTile * 4 + kHits * 2 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16);
+  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(bytes);
+  if (e != cudaSuccess) return e;
+  tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_in_place(const NsProcessArgs& a, cudaStream_t st) {
+  if (a.allowed) return launch_tiles<T, T, true>(a, st);
+  // rows longer than the table are possible only where there are that many ids
+  const bool longer = a.num_history_ids + a.num_biases > kSlots / 2;
+  const cudaError_t e = allow_smem<sparse_kernel<T>>(kRange * 4);
+  if (e != cudaSuccess) return e;
+  sparse_kernel<T><<<a.num_rows + (longer ? kHelpers : 0), kSparseThreads, kRange * 4, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -204,7 +516,7 @@ extern "C" int ns_process_logits(const NsProcessArgs* args, void* stream) {
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: fewer masks than num_rows and no allowed_rows");
   if (a.reserved != 0) return fail(NS_ERR_INVALID_ARG, "ns_process_logits: reserved must be 0");
   const int64_t blocks = (int64_t)((a.vocab_size + proc::kTile - 1) / proc::kTile) * a.num_rows;
-  if (blocks > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_process_logits: num_rows * vocab_size is too large");
+  if (blocks > 0x7fffffff - proc::kHelpers) return fail(NS_ERR_UNSUPPORTED, "ns_process_logits: num_rows * vocab_size is too large");
 
   const int64_t in_size = a.logits_dtype == NS_DTYPE_F32 ? 4 : 2, out_size = a.out_dtype == NS_DTYPE_F32 ? 4 : 2;
   const uintptr_t i0 = reinterpret_cast<uintptr_t>(a.logits), o0 = reinterpret_cast<uintptr_t>(a.out);
@@ -221,11 +533,11 @@ extern "C" int ns_process_logits(const NsProcessArgs* args, void* stream) {
   cudaError_t e;
   using bf16 = __nv_bfloat16;
   if (a.logits_dtype == NS_DTYPE_F32)
-    e = in_place ? proc::launch<float, float, true>(a, st) : proc::launch<float, float, false>(a, st);
+    e = in_place ? proc::launch_in_place<float>(a, st) : proc::launch_tiles<float, float, false>(a, st);
   else if (a.out_dtype == NS_DTYPE_F32)
-    e = proc::launch<bf16, float, false>(a, st);
+    e = proc::launch_tiles<bf16, float, false>(a, st);
   else
-    e = in_place ? proc::launch<bf16, bf16, true>(a, st) : proc::launch<bf16, bf16, false>(a, st);
+    e = in_place ? proc::launch_in_place<bf16>(a, st) : proc::launch_tiles<bf16, bf16, false>(a, st);
   if (e != cudaSuccess) return fail(NS_ERR_CUDA, std::string("ns_process_logits launch: ") + cudaGetErrorString(e));
   return NS_OK;
 }

@@ -173,6 +173,29 @@ def test_long_repetitive_histories(in_place):
     _check(NS.process_logits(x, out=x if in_place else None, **_device(d, V)), rows, d, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_in_place_with_a_few_long_rows_among_many(dtype):
+    """Rows whose ids fit the block's table, and rows that other blocks share, in one call of over 1024 rows."""
+    rng = np.random.default_rng(10)
+    S, V = 1100, 33000
+    long = {3: 5000, 600: 9001, 601: 4097, 1099: 20000}
+    hists = [rng.integers(0, V, long.get(i, int(rng.integers(0, 5)))).tolist() for i in range(S)]
+    hists[5] = rng.integers(0, V, 4096).tolist()
+    hists[6] = (np.arange(4000) * 4096 % V).tolist() + [7] * 90
+    d = dict(hists=hists, prompts=[int(rng.integers(0, len(h) + 1)) for h in hists], rep=[1.25] * S, pres=[0.5] * S,
+             freq=[0.25] * S, biases=[[(int(v), 1.5) for v in rng.choice(V, 3, replace=False)] for _ in range(S)], masks=None)
+    d["biases"][600] = [(int(v), -2.0) for v in rng.choice(V, 6000, replace=False)] + [(hists[600][0], 3.0)]
+    x = torch.from_numpy(rng.normal(0, 3, (S, V)).astype(np.float32)).to(_dev()).to(dtype)
+    kw = _device(d, V)
+    want = NS.process_logits(x, **kw)
+    pick = [0, 3, 5, 6, 600, 601, 1098, 1099]
+    rows = x[pick].double().cpu().numpy()
+    NS.process_logits(x, out=x, **kw)
+    assert torch.equal(x, want)
+    sub = {k: None if v is None else [v[i] for i in pick] for k, v in d.items()}
+    _check(x[pick], rows, sub, dtype)
+
+
 def test_a_bias_given_twice_counts_once_the_last():
     rng = np.random.default_rng(11)
     S, V = 3, 20000
