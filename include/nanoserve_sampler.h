@@ -345,7 +345,9 @@ int ns_token_logprobs(const NsLogprobArgs* args, void* stream);
  * ns_paged_history_gather: row r's prior ids out of a pool of int32 pages,
  *   out_ids[offsets[r] + j] = pool[pages[page_offsets[r] + j / page_size] * page_size + j % page_size]
  *   for j < offsets[r+1] - offsets[r]: the CSR history_ids of NsSampleArgs
- *   and NsProcessArgs.  All pointers are device pointers.  An id whose page
+ *   and NsProcessArgs.  All pointers are device pointers; offsets must not
+ *   fall (where they do, NS_STATUS_BAD_POOL_RANGE is set and some rows are
+ *   left out).  An id whose page
  *   lies outside the row's table, outside pages[num_table_pages] or outside
  *   the pool becomes -1, ids outside out_ids[num_ids] are not written; both
  *   set NS_STATUS_BAD_POOL_RANGE. */

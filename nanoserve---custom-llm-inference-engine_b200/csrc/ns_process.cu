@@ -27,8 +27,9 @@ int fail(int code, const std::string& msg);
 namespace proc {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 8192;  // multiple of 32: a tile starts on a mask word
-constexpr int kHits = 2048;
+constexpr int kTile = 12288;  // most ids of a tile
+constexpr int kSlots = 2048;  // of a tile's table, a power of two
+constexpr int kPre = 4;       // history entries per thread that are in flight at a time
 constexpr uint32_t kMaxTries = 1u << 22;
 
 // Word of one vocabulary id: occurrences after the prompt in the low bits.
@@ -91,17 +92,50 @@ __device__ __forceinline__ RowWork row_work(const NsProcessArgs& a, int row) {
   return r;
 }
 
-// f(j, id of entry j) for all n ids, kThreads apart, four loads in flight.
-template <int kBlock, typename F>
-__device__ __forceinline__ void for_ids(const int32_t* ids, int n, F f) {
-  for (int j = threadIdx.x; j < n; j += 4 * kBlock) {
-    int v[4];
+// A row's first ids, kBlock apart, on their way to registers while the block
+// clears its table: four history entries and one bias per thread.
+template <int kBlock>
+struct FirstIds {
+  int hist[kPre], bias;
+  float value;
+  __device__ __forceinline__ explicit FirstIds(const RowWork& r) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = j + u * kBlock < n ? __ldg(ids + j + u * kBlock) : -1;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (j + u * kBlock < n) f(j + u * kBlock, v[u]);
+    for (int u = 0; u < kPre; ++u) {
+      const int j = threadIdx.x + u * kBlock;
+      hist[u] = j < r.hn ? __ldg(r.hist + j) : -1;
+    }
+    bias = (int)threadIdx.x < r.bn ? __ldg(r.bias + threadIdx.x) : -1;
+    value = (int)threadIdx.x < r.bn ? __ldg(r.value + threadIdx.x) : 0.0f;
   }
+};
+
+// f(j, id) for all history entries of the row, kPre loads in flight.
+template <int kBlock, typename F>
+__device__ __forceinline__ void for_history(const RowWork& r, const FirstIds<kBlock>& first, F f) {
+  int v[kPre];
+#pragma unroll
+  for (int u = 0; u < kPre; ++u) v[u] = first.hist[u];
+  for (int j = threadIdx.x; j < r.hn;) {
+    int next[kPre];
+#pragma unroll
+    for (int u = 0; u < kPre; ++u) {
+      const int k = j + (kPre + u) * kBlock;
+      next[u] = k < r.hn ? __ldg(r.hist + k) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kPre; ++u)
+      if (j + u * kBlock < r.hn) f(j + u * kBlock, v[u]);
+    j += kPre * kBlock;
+#pragma unroll
+    for (int u = 0; u < kPre; ++u) v[u] = next[u];
+  }
+}
+
+// f(j, id, value) for all biases of the row.
+template <int kBlock, typename F>
+__device__ __forceinline__ void for_biases(const RowWork& r, const FirstIds<kBlock>& first, F f) {
+  if ((int)threadIdx.x < r.bn) f((int)threadIdx.x, first.bias, first.value);
+  for (int j = threadIdx.x + kBlock; j < r.bn; j += kBlock) f(j, __ldg(r.bias + j), __ldg(r.value + j));
 }
 
 // Entry j is the row's last for its id (asked only where an id has several).
@@ -133,25 +167,46 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar) {
   return false;
 }
 
+// Ids and their words in shared memory, open addressing.  `ids` holds id + 1, 0
+// for a free slot.
+struct Table {
+  uint32_t *ids, *words;
+  uint32_t mask;  // slots - 1
+
+  // v's slot, taken if it has none; -1 where `tries` slots in a row are others'
+  __device__ __forceinline__ int slot(uint32_t v, int tries) const {
+    uint32_t s = (v * 2654435761u) >> 12;  // golden ratio
+    for (int k = 0; k < tries; ++k, ++s) {
+      s &= mask;
+      uint32_t was = *reinterpret_cast<volatile uint32_t*>(ids + s);
+      if (was == 0) was = atomicCAS(ids + s, 0u, v + 1);
+      if (was == 0 || was == v + 1) return (int)s;
+    }
+    return -1;
+  }
+};
+constexpr int kTries = 32;
+
 // One tile of one row.  The tile is brought into shared memory by a bulk copy
-// while the block counts the row's history ids that fall into it, one 32-bit
-// word per id in shared memory (the count, a bit for the prompt, bits for
-// biases), and lists the ids it meets first.  Then each listed id's logit is
-// recomputed where it lies, and the tile leaves through a bulk copy, or, under a
-// mask or with another type, through registers.
+// while the block counts the row's history ids that fall into it in a hash
+// table in shared memory (per id the count, a bit for the prompt, bits for
+// biases).  Then each id's logit is recomputed where it lies, and the tile
+// leaves through a bulk copy, or, under a mask or with another type, through
+// registers.  Where the table is too small, its memory holds one word per id, and
+// the tile's ids are taken a part at a time.
 template <typename In, typename Out, bool kInPlace>
-__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles) {
+__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
   constexpr bool kSame = sizeof(In) == sizeof(Out);
   constexpr int kVec = 16 / sizeof(In);
   extern __shared__ __align__(128) unsigned char smem[];
-  uint32_t* words = reinterpret_cast<uint32_t*>(smem);
-  uint16_t* hits = reinterpret_cast<uint16_t*>(smem + kTile * 4);
+  const Table table{reinterpret_cast<uint32_t*>(smem), reinterpret_cast<uint32_t*>(smem) + kSlots, kSlots - 1};
+  uint32_t* direct = table.ids;  // 2 * kSlots words
   __shared__ uint64_t bar;
-  __shared__ int s_hits;
+  __shared__ int s_full;
   const int tid = threadIdx.x;
   const int row = blockIdx.x / tiles;
-  const int v0 = (blockIdx.x % tiles) * kTile;
-  const int n = min(kTile, a.vocab_size - v0);
+  const int v0 = (blockIdx.x % tiles) * width;
+  const int n = min(width, a.vocab_size - v0);
   uint32_t bad = 0;
 
   int64_t src = row;
@@ -166,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   Out* out = static_cast<Out*>(a.out) + (int64_t)row * a.out_row_stride + v0;
   // the tile in shared memory, at the same offset to the 16-byte grid as in global memory
   const int skew = (int)(reinterpret_cast<uintptr_t>(in) & 15);
-  In* x = reinterpret_cast<In*>(smem + kTile * 4 + kHits * 2 + skew);
+  In* x = reinterpret_cast<In*>(smem + kSlots * 8 + skew);
   const int head = min(n, (16 - skew) % 16 / (int)sizeof(In));  // elements before the first 16-byte boundary
   const int body = (n - head) / kVec * kVec;
   if (!kInPlace) {
@@ -182,6 +237,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
 
   const RowWork r = row_work(a, row);
   bad |= r.bad;
+  const FirstIds<kThreads> first(r);
   const uint32_t* mask = nullptr;
   if (a.allowed) {
     const int m = a.allowed_rows ? __ldg(a.allowed_rows + row) : row;
@@ -189,28 +245,81 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     else if (m >= 0) mask = reinterpret_cast<const uint32_t*>(a.allowed) + m * a.mask_stride + v0 / 32;
   }
   const int mask_words = (n + 31) / 32;
+  const auto allowed = [&](int i) { return !mask || ((__ldg(mask + (i >> 5)) >> (i & 31)) & 1u); };
   const bool counted = r.hn || r.bn;  // the same in all threads
 
-  if (tid == 0) s_hits = 0;
-  if (counted) {
-    for (int i = tid * 4; i < n; i += kThreads * 4) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    for_ids<kThreads>(r.hist, r.hn, [&](int j, int v) {
+  const auto clear = [&] {
+    uint4* t = reinterpret_cast<uint4*>(smem);
+#pragma unroll
+    for (int i = 0; i < kSlots * 8 / 16 / kThreads; ++i) t[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+  };
+  // Every history and bias entry of the tile, at the word that `word` gives for its id (null: not here).
+  const auto count = [&](auto word) {
+    for_history(r, first, [&](int j, int v) {
       if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_HISTORY_ID;
       const uint32_t i = (uint32_t)(v - v0);
-      if (i < (uint32_t)n) {
-        const uint32_t was = j < r.prompt ? atomicOr(&words[i], kInPrompt) : atomicAdd(&words[i], 1u);
-        if (!(was & (kInPrompt | kCount))) {
-          const int h = atomicAdd(&s_hits, 1);
-          if (h < kHits) hits[h] = (uint16_t)i;
-        }
+      if (i >= (uint32_t)n) return;
+      if (uint32_t* w = word(i)) {
+        if (j < r.prompt) atomicOr(w, kInPrompt);
+        else atomicAdd(w, 1u);
       }
     });
-    for_ids<kThreads>(r.bias, r.bn, [&](int, int v) {
+    for_biases(r, first, [&](int, int v, float) {
       if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_TOKEN_ID;
       const uint32_t i = (uint32_t)(v - v0);
-      if (i < (uint32_t)n && (atomicOr(&words[i], kBias) & kBias)) atomicOr(&words[i], kBiasTwice);
+      if (i >= (uint32_t)n) return;
+      if (uint32_t* w = word(i))
+        if (atomicOr(w, kBias) & kBias) atomicOr(w, kBiasTwice);
     });
+  };
+  // The results of the biased ids (one entry each computes it), and of the other id i with word w.
+  const auto fix_biased = [&](auto get, auto put, auto word) {
+    for_biases(r, first, [&](int j, int v, float value) {
+      const uint32_t i = (uint32_t)(v - v0);
+      if (i >= (uint32_t)n) return;
+      const uint32_t* w = word(i);
+      if (w && (!(*w & kBiasTwice) || last_entry(r, j, v)))
+        put((int)i, __fadd_rn(penalised(get((int)i), *w, r.pen), value));
+    });
+  };
+  const auto fix_other = [&](auto get, auto put, int i, uint32_t w) {
+    if (w && !(w & kBias)) put(i, penalised(get(i), w, r.pen));
+  };
+  const auto in_table = [&](uint32_t i) -> uint32_t* {
+    const int s = table.slot(i, kTries);
+    if (s < 0) s_full = 1;
+    return s < 0 ? nullptr : table.words + s;
+  };
+  // All of the tile's ids.  `put` is where their results go: into the tile, before it is written; or, where
+  // the tile keeps another type or is not there, to the output.
+  const auto fix = [&](auto get, auto put) {
+    if (!s_full) {
+#pragma unroll
+      for (int k = 0; k < kSlots / kThreads; ++k) {
+        const int s = k * kThreads + tid;
+        const uint32_t i = table.ids[s];
+        if (i) fix_other(get, put, (int)i - 1, table.words[s]);
+      }
+      fix_biased(get, put, in_table);
+      return;
+    }
+    for (int p0 = 0; p0 < n; p0 += 2 * kSlots) {
+      const auto word = [&](uint32_t i) { return i - p0 < 2u * kSlots ? direct + (i - p0) : nullptr; };
+      __syncthreads();
+      clear();
+      __syncthreads();
+      count(word);
+      __syncthreads();
+      for (int i = p0 + tid; i < min(n, p0 + 2 * kSlots); i += kThreads) fix_other(get, put, i, direct[i - p0]);
+      fix_biased(get, put, word);
+    }
+  };
+
+  if (counted) {
+    if (tid == 0) s_full = 0;
+    clear();
+    __syncthreads();
+    count(in_table);
   }
   __syncthreads();  // also: the barrier is initialised, the tile's ends are there
   if (!kInPlace && !wait_for(&bar)) {
@@ -218,28 +327,6 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     wait_for(&bar);  // the copy may still land
     return;
   }
-
-  // The ids that a penalty or a bias names.  `put` is where their results go: into the tile, before it is
-  // written; or, where the tile keeps another type or is not there, to the output.
-  const auto fix = [&](auto get, auto put) {
-    const auto history = [&](int i) {
-      const uint32_t w = words[i];
-      if (w && !(w & kBias)) put(i, penalised(get(i), w, r.pen));
-    };
-    const int nh = s_hits;
-    if (nh <= kHits)
-      for (int h = tid; h < nh; h += kThreads) history(hits[h]);
-    else
-      for (int i = tid; i < n; i += kThreads) history(i);
-    for_ids<kThreads>(r.bias, r.bn, [&](int j, int v) {
-      const uint32_t i = (uint32_t)(v - v0);
-      if (i >= (uint32_t)n) return;
-      const uint32_t w = words[i];
-      if (!(w & kBiasTwice) || last_entry(r, j, v))
-        put((int)i, __fadd_rn(penalised(get((int)i), w, r.pen), __ldg(r.value + j)));
-    });
-  };
-  const auto allowed = [&](int i) { return !mask || ((__ldg(mask + (i >> 5)) >> (i & 31)) & 1u); };
 
   if constexpr (kInPlace) {
     if (mask)
@@ -290,14 +377,29 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
       if (!mask && tid == 0) bulk_s2g_wait();  // shared memory is read before the block ends
     }
   } else {
-    // bf16 in, fp32 out
-    for (int i = tid * 2; i < n; i += kThreads * 2) {
-      const bool two = i + 1 < n;
-      const float y0 = allowed(i) ? load_f(x + i) : -INFINITY;
-      const float y1 = two && allowed(i + 1) ? load_f(x + i + (two ? 1 : 0)) : -INFINITY;
-      store_f(out + i, y0);
-      if (two) store_f(out + i + 1, y1);
+    // bf16 in, fp32 out: eight elements at a time from the tile's 16-byte grid
+    const auto one = [&](int i) { store_f(out + i, allowed(i) ? load_f(x + i) : -INFINITY); };
+    const bool aligned = (reinterpret_cast<uintptr_t>(out + head) & 15) == 0;
+    for (int i = head + tid * kVec; i < head + body; i += kThreads * kVec) {
+      const uint32_t bits = mask ? mask_bits(mask, mask_words, i) : ~0u;
+      const uint4 y = *reinterpret_cast<const uint4*>(x + i);
+      const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        if (!((bits >> e) & 1u)) f[e] = -INFINITY;
+      }
+      if (aligned) {
+        *reinterpret_cast<float4*>(out + i) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4*>(out + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) store_f(out + i + e, f[e]);
+      }
     }
+    if (tid < head) one(tid);
+    if (tid < n - head - body) one(head + body + tid);
     if (counted) {
       __syncthreads();
       fix([&](int i) { return load_f(x + i); },
@@ -315,15 +417,15 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
 // than the table takes are left to the kHelpers blocks behind: every one finds
 // these rows, and they share out their ranges of kRange ids, one word per id.
 constexpr int kSparseThreads = 512;
-constexpr int kSlots = 8192;  // power of two
-constexpr int kRange = 2 * kSlots;
+constexpr int kRowSlots = 8192;  // most slots of a row's table, a power of two
+constexpr int kRange = 2 * kRowSlots;
 constexpr int kHelpers = 148;
 
 template <typename T>
 __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_constant__ NsProcessArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
-  uint32_t* words = reinterpret_cast<uint32_t*>(smem);  // kSlots words and kSlots ids, or kRange words
-  uint32_t* ids = words + kSlots;                       // id + 1, 0: free
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem);  // kRowSlots words and as many ids, or kRange words
+  uint32_t* ids = words + kRowSlots;
   __shared__ uint32_t s_long[kSparseThreads / 32];
   __shared__ int s_rows[kSparseThreads];
   const int tid = threadIdx.x, lane = tid % 32;
@@ -334,21 +436,16 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
     const int row = blockIdx.x;
     const RowWork r = row_work(a, row);
     bad |= r.bad;
-    if (r.hn + r.bn > kSlots / 2) return;  // a long row
+    if (r.hn + r.bn > kRowSlots / 2) return;  // a long row
     T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_row_stride;
+    const FirstIds<kSparseThreads> first(r);
     int slots = 256;
     while (slots < 2 * (r.hn + r.bn)) slots *= 2;
     for (int i = tid; i < slots; i += kSparseThreads) words[i] = ids[i] = 0;
     __syncthreads();
-    const auto slot_of = [&](uint32_t v) {  // v's slot, taken if it has none
-      uint32_t s = (v * 2654435761u) >> 12;
-      for (;; ++s) {
-        s &= slots - 1;
-        const uint32_t was = atomicCAS(&ids[s], 0u, v + 1);  // ends: the table is at most half full
-        if (was == 0 || was == v + 1) return s;
-      }
-    };
-    for_ids<kSparseThreads>(r.hist, r.hn, [&](int j, int v) {
+    const Table table{ids, words, (uint32_t)slots - 1};
+    const auto slot_of = [&](uint32_t v) { return table.slot(v, slots); };  // found: the table is at most half full
+    for_history(r, first, [&](int j, int v) {
       if ((uint32_t)v >= V) {
         bad |= NS_STATUS_BAD_HISTORY_ID;
         return;
@@ -357,7 +454,7 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
       if (j < r.prompt) atomicOr(&words[s], kInPrompt);
       else atomicAdd(&words[s], 1u);
     });
-    for_ids<kSparseThreads>(r.bias, r.bn, [&](int, int v) {
+    for_biases(r, first, [&](int, int v, float) {
       if ((uint32_t)v >= V) {
         bad |= NS_STATUS_BAD_TOKEN_ID;
         return;
@@ -365,6 +462,7 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
       const uint32_t s = slot_of(v);
       if (atomicOr(&words[s], kBias) & kBias) atomicOr(&words[s], kBiasTwice);
     });
+    const float biased = (uint32_t)first.bias < V ? load_f(out + first.bias) : 0.0f;  // on its way
     __syncthreads();
     for (int i = tid; i < slots; i += 4 * kSparseThreads) {
       uint32_t v[4], w[4];
@@ -375,17 +473,17 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
         v[u] = s < slots ? ids[s] : 0;
         w[u] = v[u] ? words[s] : 0;
         if (w[u] & kBias) v[u] = 0;
-        y[u] = v[u] ? load_f(out + v[u] - 1) : 0.0f;
+        y[u] = v[u] ? load_f(out + (v[u] - 1)) : 0.0f;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (v[u]) store_f(out + v[u] - 1, penalised(y[u], w[u], r.pen));
+        if (v[u]) store_f(out + (v[u] - 1), penalised(y[u], w[u], r.pen));
     }
-    for_ids<kSparseThreads>(r.bias, r.bn, [&](int j, int v) {
+    for_biases(r, first, [&](int j, int v, float value) {
       if ((uint32_t)v >= V) return;
       const uint32_t w = words[slot_of(v)];
       if (!(w & kBiasTwice) || last_entry(r, j, v))
-        store_f(out + v, __fadd_rn(penalised(load_f(out + v), w, r.pen), __ldg(r.value + j)));
+        store_f(out + v, __fadd_rn(penalised(j == tid ? biased : load_f(out + v), w, r.pen), value));
     });
   } else {
     const int ranges = (a.vocab_size + kRange - 1) / kRange;
@@ -394,7 +492,7 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
       bool is_long = false;
       if (base + tid < a.num_rows) {
         const RowWork r = row_work(a, base + tid);
-        is_long = r.hn + r.bn > kSlots / 2;
+        is_long = r.hn + r.bn > kRowSlots / 2;
       }
       const uint32_t vote = __ballot_sync(0xffffffffu, is_long);
       if (lane == 0) s_long[tid / 32] = vote;
@@ -412,17 +510,18 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
         const uint32_t n = min(kRange, a.vocab_size - v0);
         const RowWork r = row_work(a, row);
         bad |= r.bad;
+        const FirstIds<kSparseThreads> first(r);
         T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_row_stride + v0;
         for (int i = tid; i < kRange; i += kSparseThreads) words[i] = 0;
         __syncthreads();
-        for_ids<kSparseThreads>(r.hist, r.hn, [&](int j, int v) {
+        for_history(r, first, [&](int j, int v) {
           if ((uint32_t)v >= V) bad |= NS_STATUS_BAD_HISTORY_ID;
           const uint32_t i = (uint32_t)(v - v0);
           if (i >= n) return;
           if (j < r.prompt) atomicOr(&words[i], kInPrompt);
           else atomicAdd(&words[i], 1u);
         });
-        for_ids<kSparseThreads>(r.bias, r.bn, [&](int, int v) {
+        for_biases(r, first, [&](int, int v, float) {
           if ((uint32_t)v >= V) bad |= NS_STATUS_BAD_TOKEN_ID;
           const uint32_t i = (uint32_t)(v - v0);
           if (i < n && (atomicOr(&words[i], kBias) & kBias)) atomicOr(&words[i], kBiasTwice);
@@ -432,12 +531,12 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_con
           const uint32_t w = words[i];
           if (w && !(w & kBias)) store_f(out + i, penalised(load_f(out + i), w, r.pen));
         }
-        for_ids<kSparseThreads>(r.bias, r.bn, [&](int j, int v) {
+        for_biases(r, first, [&](int j, int v, float value) {
           const uint32_t i = (uint32_t)(v - v0);
           if (i >= n) return;
           const uint32_t w = words[i];
           if (!(w & kBiasTwice) || last_entry(r, j, v))
-            store_f(out + i, __fadd_rn(penalised(load_f(out + i), w, r.pen), __ldg(r.value + j)));
+            store_f(out + i, __fadd_rn(penalised(load_f(out + i), w, r.pen), value));
         });
         __syncthreads();  // words may be cleared
       }
@@ -464,11 +563,19 @@ cudaError_t allow_smem(int bytes) {
 
 template <typename In, typename Out, bool kInPlace>
 cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
-  const int tiles = (a.vocab_size + kTile - 1) / kTile;
-  const int bytes = kTile * 4 + kHits * 2 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16);
-  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(bytes);
+  // Every tile of a row reads the row's history, so large batches take as few tiles as kTile allows; smaller
+  // ones need tiles of half that size to occupy the GPU (256 rows of 128256 fp32, histories of 1088: 53 us
+  // against 60; 64 rows of bf16 into fp32: 44 against 29).  All tiles are of one width, a multiple of 32: a
+  // tile starts on a mask word.
+  const int few = (a.vocab_size + kTile - 1) / kTile;
+  const int least = few * (int64_t)a.num_rows >= 148 * 8 ? few : (a.vocab_size + kTile / 2 - 1) / (kTile / 2);
+  const int width = ((a.vocab_size + least - 1) / least + 31) / 32 * 32;
+  const int tiles = (a.vocab_size + width - 1) / width;
+  const int most = kSlots * 8 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16);
+  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(most);
   if (e != cudaSuccess) return e;
-  tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles);
+  const int bytes = kSlots * 8 + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
+  tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles, width);
   return cudaGetLastError();
 }
 
@@ -476,7 +583,7 @@ template <typename T>
 cudaError_t launch_in_place(const NsProcessArgs& a, cudaStream_t st) {
   if (a.allowed) return launch_tiles<T, T, true>(a, st);
   // rows longer than the table are possible only where there are that many ids
-  const bool longer = a.num_history_ids + a.num_biases > kSlots / 2;
+  const bool longer = a.num_history_ids + a.num_biases > kRowSlots / 2;
   const cudaError_t e = allow_smem<sparse_kernel<T>>(kRange * 4);
   if (e != cudaSuccess) return e;
   sparse_kernel<T><<<a.num_rows + (longer ? kHelpers : 0), kSparseThreads, kRange * 4, st>>>(a);

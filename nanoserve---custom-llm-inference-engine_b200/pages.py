@@ -83,7 +83,8 @@ def gather_paged_history(
 
     Device tensors: ``pool`` int32 ``[num_pages, page_size]``, ``pages`` int32 (all rows' page tables,
     one after the other), ``page_offsets`` and ``history_offsets`` int64 ``[S+1]``, ``out`` int32 with room
-    for ``history_offsets[S]`` ids; ids behind them are left as they were.  Where a table is too short or a
+    for ``history_offsets[S]`` ids; ids behind them are left as they were.  Offsets must not fall (that sets
+    the status, and rows are left out).  Where a table is too short or a
     page does not exist the id becomes -1 (which the sampler reports) and ``NS_STATUS_BAD_POOL_RANGE`` is
     set in ``status`` (int32 ``[1]``).  One launch on the current stream of ``pool.device``."""
     load_ops()

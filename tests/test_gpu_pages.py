@@ -156,6 +156,26 @@ def test_gather_equals_indexing(page, rows, hi):
     assert (out[want.size:] == -7).all()
 
 
+@pytest.mark.parametrize("rows,p_empty", [(300, 0.9), (70000, 0.999), (5000, 0.0)])
+def test_gather_with_empty_and_one_id_rows(rows, p_empty):
+    """Long runs of empty rows, rows of one id, and a long row among them."""
+    rng = np.random.default_rng(rows)
+    lens = np.where(rng.random(rows) < p_empty, 0, 1)
+    lens[rows // 2] = 3000
+    need = -(-lens // 4)
+    table = rng.permutation(int(need.sum())).astype(np.int32)
+    pool = rng.integers(0, 1 << 30, (table.size, 4)).astype(np.int32)
+    po, ho = np.concatenate([[0], np.cumsum(need)]), np.concatenate([[0], np.cumsum(lens)])
+    row = np.repeat(np.arange(rows), lens)
+    j = np.arange(row.size) - ho[row]
+    want = pool[table[po[row] + j // 4], j % 4]
+    d = lambda a: torch.from_numpy(a).to(_dev())  # noqa: E731
+    out = torch.full((want.size + 700,), -7, dtype=torch.int32, device=_dev())
+    st = torch.zeros(1, dtype=torch.int32, device=_dev())
+    NS.gather_paged_history(d(pool), d(table), d(po), d(ho), out=out, status=st)
+    assert st.item() == 0 and np.array_equal(out[: want.size].cpu().numpy(), want) and (out[want.size:] == -7).all()
+
+
 def test_gather_reports_bad_tables():
     pool = torch.arange(40, dtype=torch.int32, device=_dev()).view(10, 4)
     i64 = dict(dtype=torch.int64, device=_dev())
@@ -175,7 +195,10 @@ def test_gather_reports_bad_tables():
     assert run([2], [0, 5], [0, 6], 6) == ([8, 9, 10, 11, -1, -1], bad)         # the tables end before
     assert run([2, 3], [-1, 1], [0, 5], 5) == ([-1, -1, -1, -1, 8], bad)        # a negative offset
     assert run([2, 3], [0, 2], [0, 6], 4) == ([8, 9, 10, 11], bad)              # out is too short
-    assert run([2, 3], [0, 1, 2], [0, 3, 2], 3) == ([8, 9, 10], bad)            # falling offsets
+    out, flag = run([2, 3], [0, 1, 2], [0, 3, 2], 3)                             # falling offsets: reported, in bounds
+    assert flag == bad and all(g in (w, -1, -7) for g, w in zip(out, [8, 9, 10]))
+    out, flag = run([2, 3], [0, 1, 2], [0, -9, 4], 4)
+    assert flag == bad and set(out) <= {-7, -1, *range(40)}
     assert run([2, 3], [0, 1, 2], [0, 4, 8], 8) == ([8, 9, 10, 11, 12, 13, 14, 15], 0)
 
 
