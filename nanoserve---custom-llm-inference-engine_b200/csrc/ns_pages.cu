@@ -6,7 +6,7 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -18,52 +18,91 @@ int fail(int code, const std::string& msg);
 namespace pages {
 
 constexpr int kThreads = 256;
-constexpr int kMaxBlocks = 148 * 8;
 constexpr int kMaxPools = 64;
+
+// A block copies kUnits units of one pool: the pool's moved pages one after the
+// other, cut into equal pieces, so that small pages share a block and large ones
+// are spread.  A thread has its four loads in flight together.
+constexpr int kPerThread = 4;
+constexpr int kUnits = kThreads * kPerThread;
+
+struct CopyPool {
+  char* base;
+  int64_t stride;   // bytes between pages
+  int64_t blocks;   // of the pools up to and with this one
+  uint32_t units;   // of a page
+  uint32_t unit;    // bytes: 16, 4 or 1
+};
 
 // The page numbers and pools of one launch travel as kernel parameters: no
 // staging buffer to wait for, and a captured launch keeps its own copy.
 template <int kPairs>
 struct CopyPlan {
-  NsPagePool pool[kMaxPools];
+  CopyPool pool[kMaxPools];
   int32_t src[kPairs], dst[kPairs];
   int32_t pools, pairs;
 };
 
-// Unit of all page sizes, strides and bases of the plan: 16 bytes, or 1.
-template <int kPairs, typename Unit>
-__global__ void __launch_bounds__(kThreads) copy_kernel(const __grid_constant__ CopyPlan<kPairs> p) {
-  for (int k = 0; k < p.pools; ++k) {
-    const int64_t units = p.pool[k].page_bytes / (int64_t)sizeof(Unit);
-    const int64_t stride = p.pool[k].page_stride / (int64_t)sizeof(Unit);
-    Unit* base = static_cast<Unit*>(p.pool[k].base);
-    const int64_t total = units * p.pairs;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-      const int j = (int)(i / units);
-      const int64_t u = i % units;
-      base[p.dst[j] * stride + u] = base[p.src[j] * stride + u];
+template <typename Unit, int kPairs>
+__device__ __forceinline__ void copy_block(const CopyPlan<kPairs>& p, const CopyPool& pool, int64_t block) {
+  const int64_t first = block * kUnits;
+  const int page = (int)(first / pool.units);  // the first of the block's pages
+  const uint32_t skip = (uint32_t)(first - (int64_t)page * pool.units);
+  const Unit* from[kPerThread];
+  Unit* to[kPerThread];
+  Unit v[kPerThread];
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k) {
+    const uint32_t u = skip + k * kThreads + threadIdx.x;  // below 2^32: a page has at most 2^31 units
+    const uint32_t j = page + u / pool.units, at = u % pool.units;
+    to[k] = nullptr;
+    if (j < (uint32_t)p.pairs) {
+      from[k] = reinterpret_cast<const Unit*>(pool.base + p.src[j] * pool.stride) + at;
+      to[k] = reinterpret_cast<Unit*>(pool.base + p.dst[j] * pool.stride) + at;
+      v[k] = __ldcs(from[k]);
     }
   }
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k)
+    if (to[k]) __stcs(to[k], v[k]);
 }
 
 template <int kPairs>
+__global__ void __launch_bounds__(kThreads) copy_kernel(const __grid_constant__ CopyPlan<kPairs> p) {
+  int k = 0;
+  while ((int64_t)blockIdx.x >= p.pool[k].blocks) ++k;
+  const CopyPool& pool = p.pool[k];
+  const int64_t block = blockIdx.x - (k ? p.pool[k - 1].blocks : 0);
+  if (pool.unit == 16) copy_block<uint4>(p, pool, block);
+  else if (pool.unit == 4) copy_block<uint32_t>(p, pool, block);
+  else copy_block<uint8_t>(p, pool, block);
+}
+
+// Enqueues the copies of some pools and pairs; returns how many of the pools fit
+// into the launch (at least one).
+template <int kPairs>
 cudaError_t launch(const NsPagePool* pools, int num_pools, const int64_t* src, const int64_t* dst, int count,
-                   bool wide, cudaStream_t st) {
+                   cudaStream_t st, int* taken) {
   CopyPlan<kPairs> p;
-  p.pools = num_pools;
   p.pairs = count;
-  int64_t bytes = 0;
-  for (int k = 0; k < num_pools; ++k) {
-    p.pool[k] = pools[k];
-    bytes = std::max(bytes, pools[k].page_bytes * count);
+  int64_t blocks = 0;
+  int k = 0;
+  for (; k < std::min(num_pools, kMaxPools); ++k) {
+    const NsPagePool& q = pools[k];
+    const uint64_t grid = reinterpret_cast<uintptr_t>(q.base) | (uint64_t)q.page_bytes | (uint64_t)q.page_stride;
+    const uint32_t unit = grid % 16 == 0 ? 16 : grid % 4 == 0 ? 4 : 1;
+    const int64_t units = q.page_bytes / unit, more = (units * count + kUnits - 1) / kUnits;
+    if (k > 0 && blocks + more > 0x7fffffff) break;
+    blocks += more;
+    p.pool[k] = {static_cast<char*>(q.base), q.page_stride, blocks, (uint32_t)units, unit};
   }
+  p.pools = *taken = k;
   for (int j = 0; j < count; ++j) p.src[j] = (int32_t)src[j], p.dst[j] = (int32_t)dst[j];
-  const int64_t blocks = (bytes / (wide ? 16 : 1) + kThreads - 1) / kThreads;
-  const int grid = (int)std::min<int64_t>(blocks, kMaxBlocks);
-  if (wide) copy_kernel<kPairs, uint4><<<grid, kThreads, 0, st>>>(p);
-  else copy_kernel<kPairs, uint8_t><<<grid, kThreads, 0, st>>>(p);
+  copy_kernel<kPairs><<<(unsigned)blocks, kThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
+
+thread_local std::vector<uint8_t> marks;  // one per page, all clear between calls
 
 // Empty where the plan is sound, else what is wrong with it.
 std::string check_plan(int64_t num_pages, const int64_t* src, const int64_t* dst, int64_t count) {
@@ -71,29 +110,36 @@ std::string check_plan(int64_t num_pages, const int64_t* src, const int64_t* dst
     if (src[j] < 0 || src[j] >= num_pages || dst[j] < 0 || dst[j] >= num_pages)
       return "page outside [0, " + std::to_string(num_pages) + "): " + std::to_string(src[j]) + " -> " +
              std::to_string(dst[j]);
-  std::vector<int64_t> d(dst, dst + count);
-  std::sort(d.begin(), d.end());
-  for (int64_t j = 1; j < count; ++j)
-    if (d[j] == d[j - 1]) return "page " + std::to_string(d[j]) + " is a destination twice";
-  for (int64_t j = 0; j < count; ++j)
-    if (std::binary_search(d.begin(), d.end(), src[j]))
-      return "page " + std::to_string(src[j]) + " is both a source and a destination";
-  return "";
+  if ((int64_t)marks.size() < num_pages) marks.resize(num_pages, 0);
+  std::string wrong;
+  int64_t marked = 0;
+  for (; marked < count && wrong.empty(); ++marked)
+    if (marks[dst[marked]]++) wrong = "page " + std::to_string(dst[marked]) + " is a destination twice";
+  for (int64_t j = 0; j < count && wrong.empty(); ++j)
+    if (marks[src[j]]) wrong = "page " + std::to_string(src[j]) + " is both a source and a destination";
+  while (marked > 0) marks[dst[--marked]] = 0;
+  return wrong;
 }
 
 // out[p] for every position p of the CSR array: a warp owns kChunk consecutive
 // positions, so that a few long rows and many short ones spread alike.  It finds
-// the row of its first position by a 32-way search of the offsets and walks over
-// the row ends inside the chunk; then every lane has, for each of its positions
-// (32 apart), the row and the place in it, and loads a page number and the id.
-// The chain of dependent loads (search, ends, page table, page) is what a warp
-// waits for, and integer work is what the GPU spends, so places are 32-bit.
-constexpr int kEach = 16;  // positions per lane
-constexpr int kBatch = 8;  // of these, in flight at a time
+// the row of its first position by a 32-way search of the offsets; then its lanes
+// fetch what 32 rows from there need, one each, and leave it in shared memory, and
+// every lane looks up, for each of its positions (32 apart), its row, the page
+// number and the id.  What is spent is integer work and the latency of that chain
+// of loads: places are 32-bit, and kBatch positions per lane are in flight.
+constexpr int kEach = 8;  // positions per lane
+constexpr int kBatch = 4;
 constexpr int kChunk = kEach * 32;
-constexpr int kEndBits = 9;  // kChunk = 2^9; the rows that end in a chunk fit into the other 23 bits
-constexpr int kMaxRows = 1 << 22;
-static_assert(kChunk == 1 << kEndBits, "places in a chunk");
+
+// A row as its positions in a chunk see it: position pos is place p = pos + shift
+// of the row (counted from the first page that the tables hold), on page
+// list[p / page_size] if that is below `pages`.
+struct __align__(16) RowPages {
+  const int32_t* list;
+  uint32_t pages;
+  int shift;
+};
 
 struct GatherArgs {
   const int32_t* pool;
@@ -108,7 +154,8 @@ struct GatherArgs {
   uint32_t* status;
 };
 
-__global__ void __launch_bounds__(kThreads) gather_kernel(const __grid_constant__ GatherArgs a) {
+__global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_constant__ GatherArgs a) {
+  __shared__ RowPages s_rows[kThreads / 32][32];
   const int lane = threadIdx.x % 32;
   bool bad = false;
   // every row's range, whatever the walk below makes of it
@@ -117,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const __grid_constant_
     bad |= o < 0 || e < o || e > a.num_ids || e - o > 0x7fffffff;
   }
   const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kChunk;
-  const int64_t begin = __ldg(a.offsets), end = min(__ldg(a.offsets + a.rows), a.num_ids);
+  const int64_t end = min(__ldg(a.offsets + a.rows), a.num_ids);
   if (first < end) {
     // the number of rows that end at or before `first`
     int row = 0;
@@ -129,54 +176,67 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const __grid_constant_
       row += c * step;
       n = min(step - 1, left);
     }
-    const int64_t here = __ldg(a.offsets + min(row, a.rows));  // row's first position
-    // per position: the rows that end in the chunk up to it, and the last such end (from `first`)
-    uint32_t walked[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) walked[k] = 0;
-    for (int base = row; base < a.rows; base += 32) {
-      const int64_t ends = __ldg(a.offsets + min(base + lane, a.rows - 1) + 1) - first;
-      const uint32_t inside = __ballot_sync(0xffffffffu, ends >= 0 && ends < kChunk && base + lane < a.rows);
-      const int n = __popc(inside & ~(inside + 1u));  // leading run of ends in the chunk
-      // of a whole window of empty rows only the last counts
-      const int from = n == 32 && __shfl_sync(0xffffffffu, (int)ends, 0) == __shfl_sync(0xffffffffu, (int)ends, 31) ? 31 : 0;
-      for (int k = from; k < n; ++k) {
-        const int e = __shfl_sync(0xffffffffu, (int)ends, k);
-        const uint32_t w = ((uint32_t)(base + k + 1 - row) << kEndBits) | (uint32_t)e;
-#pragma unroll
-        for (int q = 0; q < kEach; ++q)
-          if (e <= q * 32 + lane) walked[q] = w;
-      }
-      if (n < 32) break;
-    }
-    const int64_t before = first - here;  // places of `row` before the chunk
     const uint32_t size = (uint32_t)a.page_size;
-    const int shift = (size & (size - 1)) == 0 ? 31 - __clz(size) : -1;
+    const int bits = (size & (size - 1)) == 0 ? 31 - __clz(size) : -1;
+    RowPages* rows = s_rows[threadIdx.x / 32];
+    for (int base = row; base < a.rows; base += 32) {
+      const int r = min(base + lane, a.rows - 1);
+      const int64_t o = __ldg(a.offsets + r) - first, e = __ldg(a.offsets + r + 1) - first;
+      const int64_t table = __ldg(a.page_offsets + r), table_end = min(__ldg(a.page_offsets + r + 1), a.num_table);
+      const int64_t held = max(table, (int64_t)0);
+      const int64_t shift = -o - (held - table) * size;
+      RowPages mine;
+      mine.list = a.pages + held;
+      mine.pages = o <= e && shift > -0x7fffffff && shift < 0x7fffffff - kChunk
+                       ? (uint32_t)max((int64_t)0, min(table_end - held, (int64_t)0x7fffffff)) : 0u;
+      mine.shift = (int)shift;
+      __syncwarp();
+      rows[lane] = mine;
+      __syncwarp();
+      // the window's positions, and the rows that end among them
+      const int n = min(32, a.rows - base);
+      const int64_t all = __shfl_sync(0xffffffffu, e, n - 1);
+      const int from = (int)max((int64_t)0, min(__shfl_sync(0xffffffffu, o, 0), (int64_t)kChunk));
+      const int to = (int)max((int64_t)0, min(min(all, end - first), (int64_t)kChunk));
+      const int ends = __popc(__ballot_sync(0xffffffffu, e < kChunk) & (uint32_t)((1ull << n) - 1));
+      const int e32 = (int)max((int64_t)-1, min(e, (int64_t)kChunk));
+      int at[kEach];
 #pragma unroll
-    for (int k0 = 0; k0 < kEach; k0 += kBatch) {
-      int id[kBatch];
-      int64_t at[kBatch];
+      for (int k = 0; k < kEach; ++k) at[k] = 0;
+      for (int k = 0; k < min(ends, n - 1); ++k) {
+        const int x = __shfl_sync(0xffffffffu, e32, k);
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int pos = (k0 + k) * 32 + lane;
-        const uint32_t w = walked[k0 + k];
-        const int r = row + (int)(w >> kEndBits);
-        const int64_t j64 = w ? pos - (int)(w & (kChunk - 1)) : before + pos;
-        const bool here_ = r < a.rows && first + pos < end && first + pos >= begin && j64 >= 0 && j64 <= 0x7fffffff;
-        const uint32_t j = here_ ? (uint32_t)j64 : 0u;
-        const uint32_t t = shift >= 0 ? j >> shift : j / size;
-        const int64_t table = here_ ? __ldg(a.page_offsets + r) + t : 0;
-        const bool listed = here_ && table < __ldg(a.page_offsets + r + 1) && table >= 0 && table < a.num_table;
-        const int64_t page = listed ? __ldg(a.pages + table) : -1;
-        at[k] = page >= 0 && page < a.num_pages ? page * size + (j - t * size) : here_ ? -1 : -2;
+        for (int q = 0; q < kEach; ++q) at[q] += x <= q * 32 + lane;
       }
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) id[k] = at[k] >= 0 ? __ldg(a.pool + at[k]) : -1;
+      for (int k0 = 0; k0 < kEach; k0 += kBatch) {
+        uint32_t rest[kBatch];
+        int id[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (at[k] > -2) a.ids[first + (k0 + k) * 32 + lane] = id[k];
-        bad |= at[k] == -1;
+        for (int k = 0; k < kBatch; ++k) {
+          const int pos = (k0 + k) * 32 + lane;
+          const RowPages p = rows[at[k0 + k]];
+          const uint32_t place = (uint32_t)(pos + p.shift);
+          const uint32_t t = bits >= 0 ? place >> bits : place / size;
+          rest[k] = place - t * size;
+          id[k] = pos >= from && pos < to && t < p.pages ? __ldg(p.list + t) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int64_t page = id[k];
+          if (page >= 0 && page < a.num_pages) id[k] = __ldg(a.pool + (page * size + rest[k]));
+          else id[k] = -1, rest[k] = ~0u;
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int pos = (k0 + k) * 32 + lane;
+          if (pos >= from && pos < to) {
+            a.ids[first + pos] = id[k];
+            bad |= rest[k] == ~0u;
+          }
+        }
       }
+      if (all >= kChunk) break;
     }
   }
   if (bad && a.status) atomicOr(a.status, NS_STATUS_BAD_POOL_RANGE);
@@ -195,28 +255,27 @@ int ns_pages_copy(const NsPagePool* pools, int32_t num_pools, int64_t num_pages,
   if (num_pages > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_pages_copy: more than 2^31 - 1 pages");
   if (num_pools == 0 || count == 0) return NS_OK;
   if (!pools || !src || !dst) return fail(NS_ERR_INVALID_ARG, "ns_pages_copy: null pointer");
-  bool wide = true;
   for (int32_t k = 0; k < num_pools; ++k) {
     if (!pools[k].base || pools[k].page_bytes <= 0 || pools[k].page_stride < pools[k].page_bytes)
       return fail(NS_ERR_INVALID_ARG, "ns_pages_copy: pool " + std::to_string(k) +
                                           " has no base, no bytes or pages that overlap");
-    wide = wide && (reinterpret_cast<uintptr_t>(pools[k].base) | (uint64_t)pools[k].page_bytes |
-                    (uint64_t)pools[k].page_stride) % 16 == 0;
+    if (pools[k].page_bytes > 0x7fffffff)
+      return fail(NS_ERR_UNSUPPORTED, "ns_pages_copy: pages of more than 2^31 - 1 bytes");
   }
   try {
     const std::string wrong = pages::check_plan(num_pages, src, dst, count);
     if (!wrong.empty()) return fail(NS_ERR_INVALID_ARG, "ns_pages_copy: " + wrong);
-  } catch (const std::bad_alloc&) {
-    return fail(NS_ERR_INVALID_ARG, "ns_pages_copy: out of host memory");
+  } catch (const std::exception&) {  // of the marks: num_pages bytes
+    pages::marks.clear();
+    return fail(NS_ERR_UNSUPPORTED, "ns_pages_copy: out of host memory");
   }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  constexpr int kSmall = 128, kLarge = 3500;
-  for (int32_t k = 0; k < num_pools; k += pages::kMaxPools) {
-    const int np = std::min<int32_t>(pages::kMaxPools, num_pools - k);
-    for (int64_t j = 0; j < count; j += kLarge) {
-      const int n = (int)std::min<int64_t>(kLarge, count - j);
-      const cudaError_t e = n <= kSmall ? pages::launch<kSmall>(pools + k, np, src + j, dst + j, n, wide, st)
-                                        : pages::launch<kLarge>(pools + k, np, src + j, dst + j, n, wide, st);
+  constexpr int kSmall = 64, kMiddle = 512, kLarge = 3500;  // the parameters of a launch have 32764 bytes
+  for (int64_t j = 0; j < count; j += kLarge) {
+    const int n = (int)std::min<int64_t>(kLarge, count - j);
+    for (int32_t k = 0, taken = 0; k < num_pools; k += taken) {
+      const auto launch = n <= kSmall ? pages::launch<kSmall> : n <= kMiddle ? pages::launch<kMiddle> : pages::launch<kLarge>;
+      const cudaError_t e = launch(pools + k, num_pools - k, src + j, dst + j, n, st, &taken);
       if (e != cudaSuccess) return fail(NS_ERR_CUDA, std::string("ns_pages_copy launch: ") + cudaGetErrorString(e));
     }
   }
@@ -233,7 +292,6 @@ int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page
   if (num_rows == 0 || num_ids == 0) return NS_OK;
   if (!page_offsets || !offsets || !out_ids || (!pool && num_pages > 0) || (!table && num_table_pages > 0))
     return fail(NS_ERR_INVALID_ARG, "ns_paged_history_gather: null device pointer");
-  if (num_rows > pages::kMaxRows) return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: more than 2^22 rows");
   const int64_t per_block = pages::kChunk * (pages::kThreads / 32);
   const int64_t blocks = (num_ids + per_block - 1) / per_block;
   if (blocks > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: num_ids is too large");

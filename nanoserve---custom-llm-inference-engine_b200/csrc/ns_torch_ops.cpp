@@ -11,12 +11,15 @@
 // Warm a stream up before capturing a graph on it, so that the graph does
 // not hold the workspace's first zeroing.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
 #include <mutex>
+#include <tuple>
 #include <unordered_map>
 #include <vector>
 
@@ -153,6 +156,11 @@ void sample_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample
   TORCH_CHECK(rc == NS_OK, "ns_sample failed (", rc, "): ", ns_last_error());
 }
 
+void check_no_grad(const at::Tensor& t, const char* op) {
+  TORCH_CHECK(!t.requires_grad() || !c10::GradMode::is_enabled(), op,
+              " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+
 bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
 
 void check_size(const c10::optional<at::Tensor>& t, int64_t n, const char* name) {
@@ -174,9 +182,9 @@ T* opt_data(const c10::optional<at::Tensor>& t) {
   return static_cast<T*>(const_cast<void*>(opt_ptr(t)));
 }
 
-// process_logits(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
-//   presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows, out, status) -> ()
-void process_logits_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
+// process_logits_(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
+//   presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows, status, out) -> ()
+void process_logits_into(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
                        const c10::optional<at::Tensor>& history_offsets, const c10::optional<at::Tensor>& history_ids,
                        const c10::optional<at::Tensor>& prompt_lens,
                        const c10::optional<at::Tensor>& repetition_penalty,
@@ -184,10 +192,11 @@ void process_logits_op(const at::Tensor& logits, const c10::optional<at::Tensor>
                        const c10::optional<at::Tensor>& frequency_penalty,
                        const c10::optional<at::Tensor>& bias_offsets, const c10::optional<at::Tensor>& bias_ids,
                        const c10::optional<at::Tensor>& bias_values, const c10::optional<at::Tensor>& allowed,
-                       const c10::optional<at::Tensor>& allowed_rows, at::Tensor& out,
-                       const c10::optional<at::Tensor>& status) {
+                       const c10::optional<at::Tensor>& allowed_rows, const c10::optional<at::Tensor>& status,
+                       at::Tensor& out) {
   NsProcessArgs a = {};
   a.logits_dtype = check_rows(logits, "logits");
+  check_no_grad(logits, "process_logits");
   a.out_dtype = check_rows(out, "out");
   const at::Device dev = logits.device();
   c10::cuda::CUDAGuard guard(dev);
@@ -260,13 +269,35 @@ void process_logits_op(const at::Tensor& logits, const c10::optional<at::Tensor>
   TORCH_CHECK(rc == NS_OK, "ns_process_logits failed (", rc, "): ", ns_last_error());
 }
 
-// token_logprobs(logits, sample_indices, token_ids, out_logprobs, out_ranks, out_top_ids, out_top_logprobs, status) -> ()
-void token_logprobs_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
-                       const at::Tensor& token_ids, at::Tensor& out_logprobs, at::Tensor& out_ranks,
-                       at::Tensor& out_top_ids, at::Tensor& out_top_logprobs,
-                       const c10::optional<at::Tensor>& status) {
+// process_logits(logits, ..., status, out_dtype) -> a new tensor
+at::Tensor process_logits_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
+                             const c10::optional<at::Tensor>& history_offsets,
+                             const c10::optional<at::Tensor>& history_ids,
+                             const c10::optional<at::Tensor>& prompt_lens,
+                             const c10::optional<at::Tensor>& repetition_penalty,
+                             const c10::optional<at::Tensor>& presence_penalty,
+                             const c10::optional<at::Tensor>& frequency_penalty,
+                             const c10::optional<at::Tensor>& bias_offsets,
+                             const c10::optional<at::Tensor>& bias_ids, const c10::optional<at::Tensor>& bias_values,
+                             const c10::optional<at::Tensor>& allowed, const c10::optional<at::Tensor>& allowed_rows,
+                             const c10::optional<at::Tensor>& status, c10::optional<at::ScalarType> out_dtype) {
+  check_rows(logits, "logits");
+  const int64_t S = given(sample_indices) ? sample_indices->numel() : logits.size(0);
+  c10::cuda::CUDAGuard guard(logits.device());
+  at::Tensor out = at::empty({S, logits.size(1)}, logits.options().dtype(out_dtype.value_or(logits.scalar_type())));
+  process_logits_into(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
+                      presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows,
+                      status, out);
+  return out;
+}
+
+// token_logprobs(logits, sample_indices, token_ids, top_n, status) -> (logprobs, ranks, top_ids, top_logprobs)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_op(
+    const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices, const at::Tensor& token_ids,
+    int64_t n, const c10::optional<at::Tensor>& status) {
   NsLogprobArgs a = {};
   a.logits_dtype = check_rows(logits, "logits");
+  check_no_grad(logits, "token_logprobs");
   const at::Device dev = logits.device();
   c10::cuda::CUDAGuard guard(dev);
   check_cuda(token_ids, dev, "token_ids");
@@ -279,17 +310,13 @@ void token_logprobs_op(const at::Tensor& logits, const c10::optional<at::Tensor>
   check_size(sample_indices, S, "sample_indices");
   check_opt(status, dev, "status", at::kInt);
   check_size(status, 1, "status");
-  check_opt(out_logprobs, dev, "out_logprobs", at::kFloat);
-  check_size(out_logprobs, S, "out_logprobs");
-  check_opt(out_ranks, dev, "out_ranks", at::kInt);
-  check_size(out_ranks, S, "out_ranks");
-  check_opt(out_top_ids, dev, "out_top_ids", token_ids.scalar_type());
-  check_opt(out_top_logprobs, dev, "out_top_logprobs", at::kFloat);
-  TORCH_CHECK(out_top_ids.dim() == 2 && out_top_ids.size(0) == S, "out_top_ids must be [rows, top_n]");
-  const int64_t n = out_top_ids.size(1);
-  TORCH_CHECK(n <= NS_MAX_TOP_LOGPROBS && n <= V, "top_n must be at most min(vocab, ", NS_MAX_TOP_LOGPROBS, ")");
-  check_size(out_top_logprobs, S * n, "out_top_logprobs");
-  if (S == 0) return;
+  TORCH_CHECK_VALUE(n >= 0 && n <= NS_MAX_TOP_LOGPROBS && n <= V, "top_n must be between 0 and min(vocab, ",
+                    NS_MAX_TOP_LOGPROBS, "), got ", n);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor out_logprobs = at::empty({S}, f32), out_ranks = at::empty({S}, f32.dtype(at::kInt));
+  at::Tensor out_top_ids = at::empty({S, n}, token_ids.options()), out_top_logprobs = at::empty({S, n}, f32);
+  const auto result = std::make_tuple(out_logprobs, out_ranks, out_top_ids, out_top_logprobs);
+  if (S == 0) return result;
   a.logits = logits.data_ptr();
   a.vocab_size = (int32_t)V;
   a.num_logit_rows = logits.size(0);
@@ -306,6 +333,7 @@ void token_logprobs_op(const at::Tensor& logits, const c10::optional<at::Tensor>
   a.status = opt_data<uint32_t>(status);
   const int rc = ns_token_logprobs(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   TORCH_CHECK(rc == NS_OK, "ns_token_logprobs failed (", rc, "): ", ns_last_error());
+  return result;
 }
 
 // copy_pages(pools, src, dst) -> (): src and dst are CPU int64 lists of pages
@@ -316,12 +344,13 @@ void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor
   TORCH_CHECK(src.numel() == dst.numel(), "src and dst must have the same number of pages");
   if (pools.empty()) return;
   const at::Device dev = pools[0].device();
-  TORCH_CHECK(dev.is_cuda(), "pools must be CUDA tensors");
+  TORCH_CHECK(dev.is_cuda(), "copy_pages needs CUDA pools (no CPU fallback)");
   const int64_t num_pages = pools[0].dim() > 0 ? pools[0].size(0) : 0;
   std::vector<NsPagePool> p;
   p.reserve(pools.size());
   for (const at::Tensor& t : pools) {
-    TORCH_CHECK(t.is_cuda() && t.device() == dev, "pools must be on one device");
+    TORCH_CHECK(t.is_cuda() && t.device() == dev, "pools must be CUDA tensors on one device");
+    check_no_grad(t, "copy_pages");
     TORCH_CHECK(t.dim() > 0 && t.size(0) == num_pages, "pools must have the same number of pages (dimension 0)");
     int64_t elems = 1;
     bool packed = true;
@@ -386,19 +415,34 @@ TORCH_LIBRARY(nanoserve_b200, m) {
       "process_logits(Tensor logits, Tensor? sample_indices, Tensor? history_offsets, Tensor? history_ids, "
       "Tensor? prompt_lens, Tensor? repetition_penalty, Tensor? presence_penalty, Tensor? frequency_penalty, "
       "Tensor? bias_offsets, Tensor? bias_ids, Tensor? bias_values, Tensor? allowed, Tensor? allowed_rows, "
-      "Tensor(a!) out, Tensor(b!)? status=None) -> ()");
+      "Tensor(a!)? status=None, ScalarType? out_dtype=None) -> Tensor");
   m.def(
-      "token_logprobs(Tensor logits, Tensor? sample_indices, Tensor token_ids, Tensor(a!) out_logprobs, "
-      "Tensor(b!) out_ranks, Tensor(c!) out_top_ids, Tensor(d!) out_top_logprobs, Tensor(e!)? status=None) -> ()");
+      "process_logits_(Tensor logits, Tensor? sample_indices, Tensor? history_offsets, Tensor? history_ids, "
+      "Tensor? prompt_lens, Tensor? repetition_penalty, Tensor? presence_penalty, Tensor? frequency_penalty, "
+      "Tensor? bias_offsets, Tensor? bias_ids, Tensor? bias_values, Tensor? allowed, Tensor? allowed_rows, "
+      "Tensor(a!)? status, Tensor(b!) out) -> ()");
+  m.def(
+      "token_logprobs(Tensor logits, Tensor? sample_indices, Tensor token_ids, int top_n, Tensor(a!)? status=None) "
+      "-> (Tensor, Tensor, Tensor, Tensor)");
   m.def("copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst) -> ()");
   m.def(
       "paged_history_gather(Tensor pool, Tensor pages, Tensor page_offsets, Tensor history_offsets, "
       "Tensor(a!) out, Tensor(b!)? status=None) -> ()");
 }
 
+// CPU pools reach copy_pages too, for its message
+TORCH_LIBRARY_IMPL(nanoserve_b200, CPU, m) { m.impl("copy_pages", &copy_pages_op); }
+
+// these have no gradient and say so themselves: no autograd layer to go through
+TORCH_LIBRARY_IMPL(nanoserve_b200, Autograd, m) {
+  for (const char* op : {"process_logits", "process_logits_", "token_logprobs", "copy_pages", "paged_history_gather"})
+    m.impl(op, torch::CppFunction::makeFallthrough());
+}
+
 TORCH_LIBRARY_IMPL(nanoserve_b200, CUDA, m) {
   m.impl("sample", &sample_op);
   m.impl("process_logits", &process_logits_op);
+  m.impl("process_logits_", &process_logits_into);
   m.impl("token_logprobs", &token_logprobs_op);
   m.impl("copy_pages", &copy_pages_op);
   m.impl("paged_history_gather", &paged_history_gather_op);

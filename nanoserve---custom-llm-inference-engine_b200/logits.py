@@ -13,7 +13,10 @@ from typing import Optional
 
 import torch
 
-from .sampler import load_ops
+from .sampler import _Op
+
+_process = _Op("process_logits")
+_process_into = _Op("process_logits_")
 
 
 def process_logits(
@@ -68,25 +71,19 @@ def process_logits(
     Bad ids, ranges and indices are skipped and set ``NS_STATUS_*`` bits in
     ``status`` (int32 ``[1]``).  One launch on the current stream of
     ``logits.device``; no synchronisation, graph-capturable."""
-    load_ops()
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")
     if not logits.is_cuda:
         raise RuntimeError("process_logits needs CUDA logits (no CPU fallback)")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("process_logits has no gradient: call it under torch.no_grad() or on detached logits")
-    if out is None:
-        rows = logits.shape[0] if sample_indices is None else sample_indices.numel()
-        dtype = logits.dtype if out_dtype is None else out_dtype
-        if dtype not in (logits.dtype, torch.float32):
-            raise ValueError("out_dtype must be the logits' type or float32")
-        out = torch.empty(rows, logits.shape[1], dtype=dtype, device=logits.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError(f"out has dtype {out.dtype}, out_dtype is {out_dtype}")
     if logits.stride(1) != 1 and logits.shape[1] > 1 and out is not logits:
         logits = logits.contiguous()
-    torch.ops.nanoserve_b200.process_logits(
-        logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty, presence_penalty,
-        frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows, out, status,
-    )
+    given = (logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty, presence_penalty,
+             frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows, status)
+    if out is None:
+        if out_dtype not in (None, logits.dtype, torch.float32):
+            raise ValueError("out_dtype must be the logits' type or float32")
+        return _process(*given, out_dtype)
+    if out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError(f"out has dtype {out.dtype}, out_dtype is {out_dtype}")
+    _process_into(*given, out)
     return out

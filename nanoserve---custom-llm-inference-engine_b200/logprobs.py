@@ -10,7 +10,9 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _cabi
-from .sampler import load_ops
+from .sampler import _Op
+
+_token_logprobs = _Op("token_logprobs")
 
 MAX_TOP = _cabi.NS_MAX_TOP_LOGPROBS
 
@@ -44,25 +46,10 @@ def token_logprobs(
     outside ``[0, V)`` gets NaN and rank 0, and sets ``NS_STATUS_BAD_TOKEN_ID`` in
     ``status`` (int32 ``[1]``).  One launch on the current stream of
     ``logits.device``; no synchronisation, graph-capturable."""
-    load_ops()
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs needs CUDA logits (no CPU fallback)")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("token_logprobs has no gradient: call it under torch.no_grad() or on detached logits")
-    V = logits.shape[1]
-    if not 0 <= top_n <= min(V, MAX_TOP):
-        raise ValueError(f"top_n must be between 0 and min(vocab, {MAX_TOP}), got {top_n}")
-    if logits.stride(1) != 1 and V > 1:
+    if logits.stride(1) != 1 and logits.shape[1] > 1:
         logits = logits.contiguous()
-    token_ids = token_ids.contiguous()
-    S, dev = token_ids.numel(), logits.device
-    r = TokenLogprobs(
-        torch.empty(S, dtype=torch.float32, device=dev),
-        torch.empty(S, dtype=torch.int32, device=dev),
-        torch.empty(S, top_n, dtype=token_ids.dtype, device=dev),
-        torch.empty(S, top_n, dtype=torch.float32, device=dev),
-    )
-    torch.ops.nanoserve_b200.token_logprobs(logits, sample_indices, token_ids, *r, status)
-    return r
+    return TokenLogprobs(*_token_logprobs(logits, sample_indices, token_ids.contiguous(), top_n, status))

@@ -24,13 +24,18 @@ import torch
 
 from . import _cabi, packing
 from .history import StoreSampling
-from .sampler import Sampler, _Staging, load_ops, upload_parts
+from .sampler import Sampler, _Op, _Staging, load_ops, upload_parts
+
+_copy_pages = _Op("copy_pages")
+_gather = _Op("paged_history_gather")
 
 Pages = Union[Sequence[int], np.ndarray, torch.Tensor]
 
 
 def _page_list(pages: Pages, name: str) -> torch.Tensor:
     if isinstance(pages, torch.Tensor):
+        if pages.dtype == torch.int64 and pages.dim() == 1 and pages.is_cpu and pages.is_contiguous():
+            return pages
         if pages.is_cuda:
             raise RuntimeError(f"{name} must be on the host: it is checked before anything is copied")
         if pages.dtype.is_floating_point or pages.dtype.is_complex or pages.dtype == torch.bool:
@@ -54,18 +59,13 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src: Pages, d
     source and a destination.  One launch per 64 pools and 3500 pages on the
     current stream of the pools' device; the page numbers are taken during the
     call, so a graph that captures it replays the same copies."""
-    load_ops()
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     s, d = _page_list(src, "src"), _page_list(dst, "dst")
     if s.numel() != d.numel():
         raise ValueError(f"{s.numel()} source pages and {d.numel()} destination pages")
     if not pools:
         return
-    if not all(p.is_cuda for p in pools):
-        raise RuntimeError("copy_pages needs CUDA pools (no CPU fallback)")
-    if torch.is_grad_enabled() and any(p.requires_grad for p in pools):
-        raise RuntimeError("copy_pages has no gradient: pools must not require one")
-    torch.ops.nanoserve_b200.copy_pages(pools, s, d)
+    _copy_pages(pools, s, d)
 
 
 def gather_paged_history(
@@ -87,10 +87,9 @@ def gather_paged_history(
     the status, and rows are left out).  Where a table is too short or a
     page does not exist the id becomes -1 (which the sampler reports) and ``NS_STATUS_BAD_POOL_RANGE`` is
     set in ``status`` (int32 ``[1]``).  One launch on the current stream of ``pool.device``."""
-    load_ops()
     if not pool.is_cuda:
         raise RuntimeError("gather_paged_history needs a CUDA pool (no CPU fallback)")
-    torch.ops.nanoserve_b200.paged_history_gather(pool, pages, page_offsets, history_offsets, out, status)
+    _gather(pool, pages, page_offsets, history_offsets, out, status)
     return out
 
 

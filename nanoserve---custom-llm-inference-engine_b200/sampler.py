@@ -63,6 +63,20 @@ def load_ops() -> None:
     _ops_loaded = True
 
 
+class _Op:
+    """``torch.ops.nanoserve_b200.<name>``, looked up at its first call."""
+
+    def __init__(self, name: str):
+        self._name = name
+        self._op = None
+
+    def __call__(self, *args):
+        if self._op is None:
+            load_ops()
+            self._op = getattr(torch.ops.nanoserve_b200, self._name).default
+        return self._op(*args)
+
+
 class _Staging:
     """A reusable pinned host buffer plus the event of its last H2D copy."""
 
