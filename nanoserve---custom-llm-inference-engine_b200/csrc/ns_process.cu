@@ -8,7 +8,7 @@
 //   x = -inf                 where the row's mask bit is 0
 //
 // Two kernels.  tile_kernel writes whole rows (or, in place, what a mask
-// forbids): a block owns a tile of kTile vocabulary ids of one row.
+// forbids): a block owns a tile of vocabulary ids of one row.
 // sparse_kernel serves calls in place without masks, which change only the ids
 // that a history or a bias names: a block owns a row (or a part of its ids).
 #include <cuda_bf16.h>
@@ -26,9 +26,10 @@ int fail(int code, const std::string& msg);
 
 namespace proc {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 12288;  // most ids of a tile
-constexpr int kSlots = 2048;  // of a tile's table, a power of two
+constexpr int kThreads = 512;
+constexpr int kBlocks = 3;           // per SM
+constexpr int kTile = 12288;         // most ids of a tile
+constexpr int kHits = 1280;         // ids of a tile that are listed
 constexpr int kPre = 4;       // history entries per thread that are in flight at a time
 constexpr uint32_t kMaxTries = 1u << 22;
 
@@ -167,42 +168,31 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar) {
   return false;
 }
 
-// Ids and their words in shared memory, open addressing.  `ids` holds id + 1, 0
-// for a free slot.
-struct Table {
-  uint32_t *ids, *words;
-  uint32_t mask;  // slots - 1
-
-  // v's slot, taken if it has none; -1 where `tries` slots in a row are others'
-  __device__ __forceinline__ int slot(uint32_t v, int tries) const {
-    uint32_t s = (v * 2654435761u) >> 12;  // golden ratio
-    for (int k = 0; k < tries; ++k, ++s) {
-      s &= mask;
-      uint32_t was = *reinterpret_cast<volatile uint32_t*>(ids + s);
-      if (was == 0) was = atomicCAS(ids + s, 0u, v + 1);
-      if (was == 0 || was == v + 1) return (int)s;
-    }
-    return -1;
-  }
-};
-constexpr int kTries = 32;
+// A tile's ids have 16 bits each in shared memory: occurrences after the prompt
+// in the low 13 (an id that comes near their end makes the block start over with
+// 32 bits), then bits for the prompt and for biases.
+constexpr uint32_t kHalfCount = 0x1fffu, kHalfMost = 7000, kHalfBiasTwice = 0x2000u, kHalfBias = 0x4000u,
+                   kHalfPrompt = 0x8000u;
+static_assert(kHalfMost + kThreads < kHalfCount, "the count is noticed before it overflows");
+__device__ __forceinline__ uint32_t widen(uint32_t h) {
+  return (h & kHalfCount) | (h & kHalfBiasTwice ? kBiasTwice : 0u) | (h & kHalfBias ? kBias : 0u) |
+         (h & kHalfPrompt ? kInPrompt : 0u);
+}
 
 // One tile of one row.  The tile is brought into shared memory by a bulk copy
-// while the block counts the row's history ids that fall into it in a hash
-// table in shared memory (per id the count, a bit for the prompt, bits for
-// biases).  Then each id's logit is recomputed where it lies, and the tile
-// leaves through a bulk copy, or, under a mask or with another type, through
-// registers.  Where the table is too small, its memory holds one word per id, and
-// the tile's ids are taken a part at a time.
+// while the block counts the row's history ids that fall into it, 16 bits per id
+// in shared memory, and lists the ids it meets first.  Then each listed id's logit
+// is recomputed where it lies, and the tile leaves through a bulk copy, or, under a
+// mask or with another type, through registers.
 template <typename In, typename Out, bool kInPlace>
-__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
+__global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
   constexpr bool kSame = sizeof(In) == sizeof(Out);
   constexpr int kVec = 16 / sizeof(In);
   extern __shared__ __align__(128) unsigned char smem[];
-  const Table table{reinterpret_cast<uint32_t*>(smem), reinterpret_cast<uint32_t*>(smem) + kSlots, kSlots - 1};
-  uint32_t* direct = table.ids;  // 2 * kSlots words
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem);  // width 16-bit words
+  uint16_t* hits = reinterpret_cast<uint16_t*>(smem + width * 2);
   __shared__ uint64_t bar;
-  __shared__ int s_full;
+  __shared__ int s_hits, s_over;
   const int tid = threadIdx.x;
   const int row = blockIdx.x / tiles;
   const int v0 = (blockIdx.x % tiles) * width;
@@ -221,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   Out* out = static_cast<Out*>(a.out) + (int64_t)row * a.out_row_stride + v0;
   // the tile in shared memory, at the same offset to the 16-byte grid as in global memory
   const int skew = (int)(reinterpret_cast<uintptr_t>(in) & 15);
-  In* x = reinterpret_cast<In*>(smem + kSlots * 8 + skew);
+  In* x = reinterpret_cast<In*>(smem + width * 2 + kHits * 2 + skew);
   const int head = min(n, (16 - skew) % 16 / (int)sizeof(In));  // elements before the first 16-byte boundary
   const int body = (n - head) / kVec * kVec;
   if (!kInPlace) {
@@ -248,78 +238,82 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   const auto allowed = [&](int i) { return !mask || ((__ldg(mask + (i >> 5)) >> (i & 31)) & 1u); };
   const bool counted = r.hn || r.bn;  // the same in all threads
 
-  const auto clear = [&] {
-    uint4* t = reinterpret_cast<uint4*>(smem);
-#pragma unroll
-    for (int i = 0; i < kSlots * 8 / 16 / kThreads; ++i) t[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+  const auto half = [&](uint32_t i) { return (words[i >> 1] >> ((i & 1) * 16)) & 0xffffu; };
+  const auto clear = [&] {  // a width is a multiple of 32
+    for (int i = tid; i < width / 8; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   };
-  // Every history and bias entry of the tile, at the word that `word` gives for its id (null: not here).
-  const auto count = [&](auto word) {
-    for_history(r, first, [&](int j, int v) {
-      if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_HISTORY_ID;
-      const uint32_t i = (uint32_t)(v - v0);
-      if (i >= (uint32_t)n) return;
-      if (uint32_t* w = word(i)) {
-        if (j < r.prompt) atomicOr(w, kInPrompt);
-        else atomicAdd(w, 1u);
-      }
-    });
+  // Every bias entry of ids [p0, p0 + pn) of the tile: or(i, bit) sets a bit of id p0 + i and gives what was there.
+  const auto count_biases = [&](int p0, int pn, uint32_t bias, uint32_t twice, auto set) {
     for_biases(r, first, [&](int, int v, float) {
       if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_TOKEN_ID;
-      const uint32_t i = (uint32_t)(v - v0);
-      if (i >= (uint32_t)n) return;
-      if (uint32_t* w = word(i))
-        if (atomicOr(w, kBias) & kBias) atomicOr(w, kBiasTwice);
+      const uint32_t i = (uint32_t)(v - v0 - p0);
+      if (i < (uint32_t)pn && (set(i, bias) & bias)) set(i, twice);
     });
   };
-  // The results of the biased ids (one entry each computes it), and of the other id i with word w.
-  const auto fix_biased = [&](auto get, auto put, auto word) {
+  // The results of the biased ids (one entry of each computes it).
+  const auto fix_biased = [&](auto get, auto put, int p0, int pn, auto word) {
     for_biases(r, first, [&](int j, int v, float value) {
-      const uint32_t i = (uint32_t)(v - v0);
-      if (i >= (uint32_t)n) return;
-      const uint32_t* w = word(i);
-      if (w && (!(*w & kBiasTwice) || last_entry(r, j, v)))
-        put((int)i, __fadd_rn(penalised(get((int)i), *w, r.pen), value));
+      const uint32_t i = (uint32_t)(v - v0 - p0);
+      if (i >= (uint32_t)pn) return;
+      const uint32_t w = word(i);
+      if (!(w & kBiasTwice) || last_entry(r, j, v))
+        put(p0 + (int)i, __fadd_rn(penalised(get(p0 + (int)i), w, r.pen), value));
     });
   };
-  const auto fix_other = [&](auto get, auto put, int i, uint32_t w) {
-    if (w && !(w & kBias)) put(i, penalised(get(i), w, r.pen));
-  };
-  const auto in_table = [&](uint32_t i) -> uint32_t* {
-    const int s = table.slot(i, kTries);
-    if (s < 0) s_full = 1;
-    return s < 0 ? nullptr : table.words + s;
-  };
-  // All of the tile's ids.  `put` is where their results go: into the tile, before it is written; or, where
-  // the tile keeps another type or is not there, to the output.
+  // All ids of the tile that a penalty or a bias names.  `put` is where their results go: into the tile, before
+  // it is written; or, where the tile keeps another type or is not there, to the output.
   const auto fix = [&](auto get, auto put) {
-    if (!s_full) {
-#pragma unroll
-      for (int k = 0; k < kSlots / kThreads; ++k) {
-        const int s = k * kThreads + tid;
-        const uint32_t i = table.ids[s];
-        if (i) fix_other(get, put, (int)i - 1, table.words[s]);
-      }
-      fix_biased(get, put, in_table);
+    const auto history = [&](int i, uint32_t w) {
+      if (w && !(w & kBias)) put(i, penalised(get(i), w, r.pen));
+    };
+    if (!s_over) {
+      const int nh = s_hits;
+      if (nh <= kHits)
+        for (int h = tid; h < nh; h += kThreads) history(hits[h], widen(half(hits[h])));
+      else
+        for (int i = tid; i < n; i += kThreads) history(i, widen(half(i)));
+      fix_biased(get, put, 0, n, [&](uint32_t i) { return widen(half(i)); });
       return;
     }
-    for (int p0 = 0; p0 < n; p0 += 2 * kSlots) {
-      const auto word = [&](uint32_t i) { return i - p0 < 2u * kSlots ? direct + (i - p0) : nullptr; };
+    const int part = width / 2;  // ids that the same memory holds in 32 bits
+    for (int p0 = 0; p0 < n; p0 += part) {
+      const int pn = min(part, n - p0);
       __syncthreads();
       clear();
       __syncthreads();
-      count(word);
+      for_history(r, first, [&](int j, int v) {
+        const uint32_t i = (uint32_t)(v - v0 - p0);
+        if (i >= (uint32_t)pn) return;
+        if (j < r.prompt) atomicOr(&words[i], kInPrompt);
+        else atomicAdd(&words[i], 1u);
+      });
+      count_biases(p0, pn, kBias, kBiasTwice, [&](uint32_t i, uint32_t bit) { return atomicOr(&words[i], bit); });
       __syncthreads();
-      for (int i = p0 + tid; i < min(n, p0 + 2 * kSlots); i += kThreads) fix_other(get, put, i, direct[i - p0]);
-      fix_biased(get, put, word);
+      for (int i = tid; i < pn; i += kThreads) history(p0 + i, words[i]);
+      fix_biased(get, put, p0, pn, [&](uint32_t i) { return words[i]; });
     }
   };
 
   if (counted) {
-    if (tid == 0) s_full = 0;
+    if (tid == 0) s_hits = s_over = 0;
     clear();
     __syncthreads();
-    count(in_table);
+    for_history(r, first, [&](int j, int v) {
+      if ((uint32_t)v >= (uint32_t)a.vocab_size) bad |= NS_STATUS_BAD_HISTORY_ID;
+      const uint32_t i = (uint32_t)(v - v0);
+      if (i >= (uint32_t)n) return;
+      const int sh = (i & 1) * 16;
+      const uint32_t was = (j < r.prompt ? atomicOr(&words[i >> 1], kHalfPrompt << sh) : atomicAdd(&words[i >> 1], 1u << sh)) >> sh;
+      if (!(was & (kHalfPrompt | kHalfCount))) {
+        const int h = atomicAdd(&s_hits, 1);
+        if (h < kHits) hits[h] = (uint16_t)i;
+      }
+      if ((was & kHalfCount) >= kHalfMost) s_over = 1;
+    });
+    count_biases(0, n, kHalfBias, kHalfBiasTwice, [&](uint32_t i, uint32_t bit) {
+      const int sh = (i & 1) * 16;
+      return atomicOr(&words[i >> 1], bit << sh) >> sh;
+    });
   }
   __syncthreads();  // also: the barrier is initialised, the tile's ends are there
   if (!kInPlace && !wait_for(&bar)) {
@@ -411,15 +405,33 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   if (bad && a.status) atomicOr(a.status, bad);
 }
 
+// Ids and their words in shared memory, open addressing.  `ids` holds id + 1, 0
+// for a free slot.
+struct Table {
+  uint32_t *ids, *words;
+  uint32_t mask;  // slots - 1
+
+  // v's slot, taken if it has none; -1 where `tries` slots in a row are others'
+  __device__ __forceinline__ int slot(uint32_t v, int tries) const {
+    uint32_t s = (v * 2654435761u) >> 12;  // golden ratio
+    for (int k = 0; k < tries; ++k, ++s) {
+      s &= mask;
+      uint32_t was = *reinterpret_cast<volatile uint32_t*>(ids + s);
+      if (was == 0) was = atomicCAS(ids + s, 0u, v + 1);
+      if (was == 0 || was == v + 1) return (int)s;
+    }
+    return -1;
+  }
+};
 // In place and without masks only the ids that a history or a bias names
 // change.  Block `row` counts its row's ids in a hash table in shared memory (open
 // addressing, at most half full) and recomputes each once.  Rows with more ids
 // than the table takes are left to the kHelpers blocks behind: every one finds
 // these rows, and they share out their ranges of kRange ids, one word per id.
-constexpr int kSparseThreads = 512;
+constexpr int kSparseThreads = 1024;
 constexpr int kRowSlots = 8192;  // most slots of a row's table, a power of two
 constexpr int kRange = 2 * kRowSlots;
-constexpr int kHelpers = 148;
+constexpr int kHelpers = 32;
 
 template <typename T>
 __global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_constant__ NsProcessArgs a) {
@@ -563,18 +575,18 @@ cudaError_t allow_smem(int bytes) {
 
 template <typename In, typename Out, bool kInPlace>
 cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
-  // Every tile of a row reads the row's history, so large batches take as few tiles as kTile allows; smaller
-  // ones need tiles of half that size to occupy the GPU (256 rows of 128256 fp32, histories of 1088: 53 us
-  // against 60; 64 rows of bf16 into fp32: 44 against 29).  All tiles are of one width, a multiple of 32: a
-  // tile starts on a mask word.
-  const int few = (a.vocab_size + kTile - 1) / kTile;
-  const int least = few * (int64_t)a.num_rows >= 148 * 8 ? few : (a.vocab_size + kTile / 2 - 1) / (kTile / 2);
-  const int width = ((a.vocab_size + least - 1) / least + 31) / 32 * 32;
+  // Every tile of a row reads the row's history and waits for its loads in turn, so a row has as few tiles as
+  // possible; where all blocks fit on the GPU at once, as many as do.  (256 rows of 128256 fp32 with histories
+  // of about 1088: 47 us in 11 tiles, 60 in 21; 64 rows of bf16 into fp32 with histories of about 2300: TBD us in 6
+  // tiles, 29 in 21.)  All tiles are of one width, a multiple of 32: a tile starts on a mask word.
+  const int64_t least = (a.vocab_size + kTile - 1) / kTile;
+  const int64_t fit = std::min<int64_t>(148 * kBlocks / a.num_rows, a.vocab_size / 2048);
+  const int64_t wanted = std::max(least, fit);
+  const int width = (int)((a.vocab_size + wanted - 1) / wanted + 31) / 32 * 32;
   const int tiles = (a.vocab_size + width - 1) / width;
-  const int most = kSlots * 8 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16);
-  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(most);
+  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(kTile * 2 + kHits * 2 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16));
   if (e != cudaSuccess) return e;
-  const int bytes = kSlots * 8 + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
+  const int bytes = width * 2 + kHits * 2 + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
   tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles, width);
   return cudaGetLastError();
 }
