@@ -8,11 +8,11 @@
 // One pass over the logits gives every sum: a cluster of C blocks takes a row
 // (C by the number of rows, so that few rows still fill the GPU), each block a
 // contiguous slice of it, each thread every 256th 16-byte vector of the slice
-// (its bucket).  A thread keeps its bucket's maximum, its sum of exponentials
-// over a reference that follows the maximum in steps, and its count of larger
-// logits.  The n largest are then in few buckets: those whose maximum reaches
-// the n-th largest bucket maximum.  Only these are read again (out of L2); the
-// elements that reach the bound are ranked by counting (or, where ties make
+// (its bucket).  A thread keeps the maxima of its batches, its sum of
+// exponentials over a reference that follows the maximum in steps, and its count
+// of larger logits.  The n largest are then in few batches: those whose maximum
+// reaches a bound that n buckets reach.  Only these are read again (out of L2);
+// the elements that reach the bound are ranked by counting (or, where ties make
 // them many, through sorted lists), within the block and then, through
 // distributed shared memory, within the cluster.
 #include <cuda_bf16.h>
@@ -34,9 +34,11 @@ constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
 constexpr int kMaxCluster = 8;     // the portable limit
 constexpr float kLag = 8.0f;       // the reference follows the maximum in steps of at least this
 constexpr float kHuge = 0x1p100f;  // beyond it the fused argument of the exponential could overflow
+constexpr int kEntries = 32;       // maxima that a thread keeps
+constexpr int kListed = 512;       // entries that are read again
 constexpr int kCands = 256;        // candidates that are ranked by counting
 typedef unsigned long long u64;
-static_assert(kMaxCluster * NS_MAX_TOP_LOGPROBS <= kThreads, "the cluster's lists fit into s_list");
+static_assert(kMaxCluster * NS_MAX_TOP_LOGPROBS <= kThreads, "every thread ranks one key of the cluster's");
 
 // Larger value first, then smaller id, as one key to maximise; -0 counts as 0.
 // No logit's key is 0.
@@ -200,11 +202,15 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   __shared__ float s_max[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_cnt[kWarps];
-  __shared__ uint32_t s_few[kWarps], s_bound;
-  __shared__ int s_buckets, s_cands;
-  __shared__ u64 s_list[kThreads];  // buckets, then sorted keys
+  __shared__ uint32_t s_entry[kEntries][kThreads];
+  __shared__ uint32_t s_few[kWarps];
+  __shared__ uint16_t s_list[kListed];
+  __shared__ int s_listed, s_cands;
+  __shared__ u64 s_best[kThreads];  // sorted keys: the warps', then the block's, then the row's
   __shared__ u64 s_cand[kCands];
+  __shared__ u64 s_remote[(kMaxCluster - 1) * NS_MAX_TOP_LOGPROBS];  // the other blocks' keys and parts
   __shared__ Part s_part[kMaxCluster];
+  if (C > 1) cluster_arrive_relaxed();  // this block runs: its shared memory may be written
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int row = blockIdx.x / C, rank = blockIdx.x % C;
   const int V = a.vocab_size, n = a.top_n;
@@ -232,9 +238,24 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   const int lo = (int)((int64_t)vecs * rank / C), hi = (int)((int64_t)vecs * (rank + 1) / C);
   const In* xv = x + head;
 
+  // Batches of kUnroll vectors per thread, then what is left of its vectors.  The key of each batch's (or, in
+  // long slices, of each `group` batches') maximum stays in shared memory; the one largest element alone is
+  // found well enough from the maximum of all.
+  const int batches = (hi - lo + kUnroll * kThreads - 1) / (kUnroll * kThreads);
+  const int group = n > 1 ? (batches + kEntries - 1) / kEntries : batches;
   Sum sum;
   typename R::Count count(xt);
   float m = -INFINITY;
+  uint32_t bucket = 0, entry = 0;  // keys of maxima: this thread's, and the current entry's (0: nothing)
+  int entries = 0, in_entry = 0;
+  const auto note = [&](float bm) {
+    entry = max(entry, f2key(bm + 0.0f));
+    if (++in_entry == group) {
+      s_entry[entries++][tid] = entry;
+      bucket = max(bucket, entry);
+      entry = 0, in_entry = 0;
+    }
+  };
   int i = lo + tid;
   for (; i + (kUnroll - 1) * kThreads < hi; i += kUnroll * kThreads) {
     Vec b[kUnroll];
@@ -242,19 +263,30 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
     for (int u = 0; u < kUnroll; ++u) b[u].load(xv + (int64_t)(i + u * kThreads) * kVec);
     const float bm = R::max_of(b);
     m = fmax_nan(m, bm);
+    if (n > 1) note(bm);
     count.add(b);
     sum.template add<R>(b, bm);
   }
+  float rest = -INFINITY;
+  const bool some = i < hi;
   for (; i < hi; i += kThreads) {
     Vec b[1];
     b[0].load(xv + (int64_t)i * kVec);
     const float bm = R::max_of(b);
-    m = fmax_nan(m, bm);
+    rest = fmax_nan(rest, bm);
     count.add(b);
     sum.template add<R>(b, bm);
   }
-  // this thread's bucket: vectors lo + tid, lo + tid + kThreads, ...
-  const uint32_t bucket = lo + tid < hi ? f2key(m + 0.0f) : 0u;
+  m = fmax_nan(m, rest);
+  if (n == 1 && lo + tid < hi) {
+    entry = f2key(m + 0.0f);
+  } else if (n > 1 && some) {
+    entry = max(entry, f2key(rest + 0.0f));
+  }
+  if (n > 0) {
+    if (entry) s_entry[entries++][tid] = entry;
+    bucket = max(bucket, entry);
+  }
   int cnt = count.total();
   // the elements off the 16-byte grid: one each for threads of the first block
   const int odd = rank == 0 && tid < head + tail ? (tid < head ? tid : V - tail + tid - head) : -1;
@@ -281,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
       if (__ffs(__ballot_sync(0xffffffffu, left == few)) - 1 == lane) left = 0;
     }
     if (lane == 0) s_few[warp] = few;
-    if (tid == 0) s_buckets = s_cands = 0;
+    if (tid == 0) s_listed = s_cands = 0;
   }
   if (lane == 0) s_max[warp] = bm, s_cnt[warp] = cnt;
   __syncthreads();
@@ -292,65 +324,40 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   if (lane == 0) s_sum[warp] = part;
 
   if (n > 0) {
-    // n buckets reach the least of the warps' q-th maxima: list the buckets that do, and find the
-    // n-th largest maximum (0 if there are fewer) among them
-    uint32_t few = s_few[0];
+    // n buckets reach the least of the warps' q-th maxima, so the n largest elements reach it too: list the
+    // entries that do, and read them again
+    uint32_t bound = s_few[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) few = n == 1 ? max(few, s_few[w]) : min(few, s_few[w]);
-    if (bucket && bucket >= few) s_list[atomicAdd(&s_buckets, 1)] = ((u64)bucket << 32) | (uint32_t)tid;
-    if (tid == 0) s_bound = few;
-    __syncthreads();
-    const int nb = s_buckets;
-    if (n > 1 && tid < nb) {
-      const uint32_t mine = (uint32_t)(s_list[tid] >> 32);
-      int more = 0, same = 0;
-      for (int j = 0; j < nb; ++j) {
-        const uint32_t k = (uint32_t)(s_list[j] >> 32);
-        more += k > mine, same += k == mine;
-      }
-      if (more < n && n <= more + same) s_bound = mine;  // one value, whoever writes it
-    }
-    __syncthreads();
-    // every element that reaches the bound is in one of these buckets: read them again
-    const u64 bound = (u64)s_bound << 32;
-    const int chunks = (hi - lo + 32 * kThreads - 1) / (32 * kThreads);
-    const int items = nb * chunks;
-    for (int k = warp; k < items; k += kWarps * kUnroll) {
-      Vec b[kUnroll];
-      int at[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int item = k + u * kWarps;
-        at[u] = -1;
-        if (item < items) {
-          const u64 e = s_list[item / chunks];
-          const int j = lo + (int)(uint32_t)e + ((item % chunks) * 32 + lane) * kThreads;
-          if (e >= bound && j < hi) at[u] = j;
+    for (int w = 1; w < kWarps; ++w) bound = n == 1 ? max(bound, s_few[w]) : min(bound, s_few[w]);
+    if (bucket && bucket >= bound)
+      for (int e = 0; e < entries; ++e)
+        if (s_entry[e][tid] >= bound) {
+          const int k = atomicAdd(&s_listed, 1);
+          if (k < kListed) s_list[k] = (uint16_t)(e * kThreads + tid);
         }
-        if (at[u] >= 0) b[u].load(xv + (int64_t)at[u] * kVec);
-      }
+    const float least = bound ? key2f(bound) : -INFINITY;
+    if (odd_key && (uint32_t)(odd_key >> 32) >= bound) s_cand[atomicAdd(&s_cands, 1)] = odd_key;
+    __syncthreads();
+    const int listed = s_listed;
+    if (listed <= kListed)
+      for (int q = tid; q < listed * group * kUnroll; q += kThreads) {
+        const int e = s_list[q / (group * kUnroll)];
+        const int j = lo + (e / kThreads * group * kUnroll + q % (group * kUnroll)) * kThreads + e % kThreads;
+        if (j >= hi) continue;
+        Vec y;
+        y.load(xv + (int64_t)j * kVec);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (at[u] < 0) continue;
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const u64 key = top_key(b[u].get(e), head + at[u] * kVec + e);
-          if (key >= bound) {
+        for (int k = 0; k < kVec; ++k)
+          if (y.get(k) >= least) {
             const int c = atomicAdd(&s_cands, 1);
-            if (c < kCands) s_cand[c] = key;
+            if (c < kCands) s_cand[c] = top_key(y.get(k), head + j * kVec + k);
           }
-        }
       }
-    }
-    if (odd_key >= bound && odd_key) {
-      const int c = atomicAdd(&s_cands, 1);
-      if (c < kCands) s_cand[c] = odd_key;
-    }
     __syncthreads();
     const int nc = s_cands;
     u64 mine = 0;
     int place = 32;
-    if (nc <= kCands) {
+    if (listed <= kListed && nc <= kCands) {
       // few candidates: each counts the larger ones
       if (tid < nc) {
         mine = s_cand[tid];
@@ -363,12 +370,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
       u64 list = 0;
       for (uint32_t take = __ballot_sync(0xffffffffu, odd_key != 0); take; take &= take - 1)
         list = insert(list, __shfl_sync(0xffffffffu, odd_key, __ffs(take) - 1), lane);
-      for (int k = warp; k < nb; k += kWarps) {
-        const u64 e = s_list[k];
-        if (e < bound) continue;
-        const int first = lo + (int)(uint32_t)e;  // the bucket's first vector
+      for (uint32_t left = __ballot_sync(0xffffffffu, bucket && bucket >= bound); left; left &= left - 1) {
+        const int owner = __ffs(left) - 1;
+        const int first = lo + warp * 32 + owner;  // the bucket's first vector
+        const u64 best = ((u64)__shfl_sync(0xffffffffu, bucket, owner) << 32) | (uint32_t)~(head + first * kVec);
         u64 nth = __shfl_sync(0xffffffffu, list, n - 1);
-        if (((e >> 32 << 32) | (uint32_t)~(head + first * kVec)) <= nth) continue;
+        if (best <= nth) continue;
         for (int j = first; j < hi; j += 32 * kThreads) {
           const int at = j + lane * kThreads;
           Vec b;
@@ -386,23 +393,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
           }
         }
       }
-      __syncthreads();  // the buckets have been read
-      s_list[tid] = list;
+      s_best[tid] = list;
 #pragma unroll
       for (int s = 1; s < kWarps; s <<= 1) {
         __syncthreads();
         if (warp % (2 * s) == 0) {
-          list = merge_lists(list, s_list[(warp + s) * 32 + lane], lane);
-          s_list[tid] = list;
+          list = merge_lists(list, s_best[(warp + s) * 32 + lane], lane);
+          s_best[tid] = list;
         }
       }
       if (warp == 0) mine = list, place = lane;
     }
     // the block's best n, in order; a slice with fewer elements leaves zeros
     __syncthreads();
-    if (tid < 32) s_list[tid] = 0;
+    if (tid < 32) s_best[tid] = 0;
     __syncthreads();
-    if (place < n) s_list[place] = mine;
+    if (place < n) s_best[place] = mine;
   }
   __syncthreads();
   Part p;
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   }
   if (C > 1) {
     // every block's part and list to the first block of the cluster
-    cluster_sync();  // every block of the cluster runs and is done with its lists
+    cluster_wait();
     if (warp == 0 && rank != 0) {
       const uint32_t to = dsmem_map(smem_addr(&s_part[rank]), 0);
       if (lane == 0) {
@@ -420,22 +426,23 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
         dsmem_st_f32(to + offsetof(Part, max), p.max);
         dsmem_st_u32(to + offsetof(Part, count), (uint32_t)p.count);
       }
-      if (lane < n) dsmem_st_u64(dsmem_map(smem_addr(&s_list[rank * n + lane]), 0), s_list[lane]);
+      if (lane < n) dsmem_st_u64(dsmem_map(smem_addr(&s_remote[(rank - 1) * n + lane]), 0), s_best[lane]);
     }
     cluster_sync();
     if (rank != 0) return;
     if (n > 0) {
       // each of the blocks' best counts the larger ones
-      const u64 mine = tid < C * n ? s_list[tid] : 0;
+      const u64 mine = tid < n ? s_best[tid] : tid < C * n ? s_remote[tid - n] : 0;
       int place = 0;
-      for (int j = 0; j < C * n; ++j) place += s_list[j] > mine;
+      for (int j = 0; j < n; ++j) place += s_best[j] > mine;
+      for (int j = 0; j < (C - 1) * n; ++j) place += s_remote[j] > mine;
       __syncthreads();
-      if (mine && place < n) s_list[place] = mine;
+      if (mine && place < n) s_best[place] = mine;
       __syncthreads();
     }
   }
   if (warp != 0) return;
-  const u64 list = lane < n ? s_list[lane] : 0;
+  const u64 list = lane < n ? s_best[lane] : 0;
   float top = p.max;
   for (int c = 1; c < C; ++c) top = fmax_nan(top, s_part[c].max), p.count += s_part[c].count;
   const bool uniform = !(fabsf(top) < INFINITY);  // NaN, +inf, or only -inf

@@ -29,7 +29,9 @@ namespace proc {
 constexpr int kThreads = 512;
 constexpr int kBlocks = 3;           // per SM
 constexpr int kTile = 12288;         // most ids of a tile
-constexpr int kHits = 1280;         // ids of a tile that are listed
+// ids of a tile that are listed (three blocks of the largest tiles share an SM's memory)
+template <typename In>
+constexpr int kHits = sizeof(In) == 4 ? 1280 : 4096;
 constexpr int kPre = 4;       // history entries per thread that are in flight at a time
 constexpr uint32_t kMaxTries = 1u << 22;
 
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_co
   Out* out = static_cast<Out*>(a.out) + (int64_t)row * a.out_row_stride + v0;
   // the tile in shared memory, at the same offset to the 16-byte grid as in global memory
   const int skew = (int)(reinterpret_cast<uintptr_t>(in) & 15);
-  In* x = reinterpret_cast<In*>(smem + width * 2 + kHits * 2 + skew);
+  In* x = reinterpret_cast<In*>(smem + width * 2 + kHits<In> * 2 + skew);
   const int head = min(n, (16 - skew) % 16 / (int)sizeof(In));  // elements before the first 16-byte boundary
   const int body = (n - head) / kVec * kVec;
   if (!kInPlace) {
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_co
     };
     if (!s_over) {
       const int nh = s_hits;
-      if (nh <= kHits)
+      if (nh <= kHits<In>)
         for (int h = tid; h < nh; h += kThreads) history(hits[h], widen(half(hits[h])));
       else
         for (int i = tid; i < n; i += kThreads) history(i, widen(half(i)));
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_co
       const uint32_t was = (j < r.prompt ? atomicOr(&words[i >> 1], kHalfPrompt << sh) : atomicAdd(&words[i >> 1], 1u << sh)) >> sh;
       if (!(was & (kHalfPrompt | kHalfCount))) {
         const int h = atomicAdd(&s_hits, 1);
-        if (h < kHits) hits[h] = (uint16_t)i;
+        if (h < kHits<In>) hits[h] = (uint16_t)i;
       }
       if ((was & kHalfCount) >= kHalfMost) s_over = 1;
     });
@@ -577,16 +579,15 @@ template <typename In, typename Out, bool kInPlace>
 cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
   // Every tile of a row reads the row's history and waits for its loads in turn, so a row has as few tiles as
   // possible; where all blocks fit on the GPU at once, as many as do.  (256 rows of 128256 fp32 with histories
-  // of about 1088: 47 us in 11 tiles, 60 in 21; 64 rows of bf16 into fp32 with histories of about 2300: TBD us in 6
-  // tiles, 29 in 21.)  All tiles are of one width, a multiple of 32: a tile starts on a mask word.
+  // of about 1088: 46 us in 11 tiles, 62 in 21.)  All tiles are of one width, a multiple of 32: a tile starts on a mask word.
   const int64_t least = (a.vocab_size + kTile - 1) / kTile;
   const int64_t fit = std::min<int64_t>(148 * kBlocks / a.num_rows, a.vocab_size / 2048);
   const int64_t wanted = std::max(least, fit);
   const int width = (int)((a.vocab_size + wanted - 1) / wanted + 31) / 32 * 32;
   const int tiles = (a.vocab_size + width - 1) / width;
-  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(kTile * 2 + kHits * 2 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16));
+  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(kTile * 2 + kHits<In> * 2 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16));
   if (e != cudaSuccess) return e;
-  const int bytes = width * 2 + kHits * 2 + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
+  const int bytes = width * 2 + kHits<In> * 2 + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
   tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles, width);
   return cudaGetLastError();
 }
