@@ -169,8 +169,8 @@ void check_size(const c10::optional<at::Tensor>& t, int64_t n, const char* name)
 
 // fp32 or bf16 rows; returns NS_DTYPE_*
 int32_t check_rows(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.dim() == 2, name, " must be 2-D [rows, vocab]");
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (no CPU fallback)");
+  TORCH_CHECK_VALUE(t.dim() == 2, name, " must be [rows, vocab]");
   TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " rows must be contiguous");
   TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, " must be float32 or bfloat16");
   TORCH_CHECK(t.size(1) > 0 && t.size(1) <= INT32_MAX, name, " must have between 1 and 2^31 - 1 columns");
@@ -269,8 +269,13 @@ void process_logits_into(const at::Tensor& logits, const c10::optional<at::Tenso
   TORCH_CHECK(rc == NS_OK, "ns_process_logits failed (", rc, "): ", ns_last_error());
 }
 
+// Rows whose elements are next to each other (a copy of columns that are not).
+at::Tensor packed_rows(const at::Tensor& t) {
+  return t.dim() == 2 && t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
+}
+
 // process_logits(logits, ..., status, out_dtype) -> a new tensor
-at::Tensor process_logits_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
+at::Tensor process_logits_op(const at::Tensor& given_logits, const c10::optional<at::Tensor>& sample_indices,
                              const c10::optional<at::Tensor>& history_offsets,
                              const c10::optional<at::Tensor>& history_ids,
                              const c10::optional<at::Tensor>& prompt_lens,
@@ -281,7 +286,10 @@ at::Tensor process_logits_op(const at::Tensor& logits, const c10::optional<at::T
                              const c10::optional<at::Tensor>& bias_ids, const c10::optional<at::Tensor>& bias_values,
                              const c10::optional<at::Tensor>& allowed, const c10::optional<at::Tensor>& allowed_rows,
                              const c10::optional<at::Tensor>& status, c10::optional<at::ScalarType> out_dtype) {
+  const at::Tensor logits = packed_rows(given_logits);
   check_rows(logits, "logits");
+  TORCH_CHECK_VALUE(!out_dtype || *out_dtype == logits.scalar_type() || *out_dtype == at::kFloat,
+                    "out_dtype must be the logits' type or float32");
   const int64_t S = given(sample_indices) ? sample_indices->numel() : logits.size(0);
   c10::cuda::CUDAGuard guard(logits.device());
   at::Tensor out = at::empty({S, logits.size(1)}, logits.options().dtype(out_dtype.value_or(logits.scalar_type())));
@@ -293,8 +301,9 @@ at::Tensor process_logits_op(const at::Tensor& logits, const c10::optional<at::T
 
 // token_logprobs(logits, sample_indices, token_ids, top_n, status) -> (logprobs, ranks, top_ids, top_logprobs)
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_op(
-    const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices, const at::Tensor& token_ids,
-    int64_t n, const c10::optional<at::Tensor>& status) {
+    const at::Tensor& given_logits, const c10::optional<at::Tensor>& sample_indices,
+    const at::Tensor& given_ids, int64_t n, const c10::optional<at::Tensor>& status) {
+  const at::Tensor logits = packed_rows(given_logits), token_ids = given_ids.contiguous();
   NsLogprobArgs a = {};
   a.logits_dtype = check_rows(logits, "logits");
   check_no_grad(logits, "token_logprobs");
@@ -341,7 +350,7 @@ void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor
   TORCH_CHECK(src.device().is_cpu() && dst.device().is_cpu() && src.scalar_type() == at::kLong &&
                   dst.scalar_type() == at::kLong && src.is_contiguous() && dst.is_contiguous(),
               "src and dst must be contiguous int64 CPU tensors");
-  TORCH_CHECK(src.numel() == dst.numel(), "src and dst must have the same number of pages");
+  TORCH_CHECK_VALUE(src.numel() == dst.numel(), src.numel(), " source pages and ", dst.numel(), " destination pages");
   if (pools.empty()) return;
   const at::Device dev = pools[0].device();
   TORCH_CHECK(dev.is_cuda(), "copy_pages needs CUDA pools (no CPU fallback)");
@@ -380,7 +389,7 @@ void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor
 void paged_history_gather_op(const at::Tensor& pool, const at::Tensor& pages, const at::Tensor& page_offsets,
                              const at::Tensor& history_offsets, at::Tensor& out,
                              const c10::optional<at::Tensor>& status) {
-  TORCH_CHECK(pool.is_cuda(), "pool must be a CUDA tensor");
+  TORCH_CHECK(pool.is_cuda(), "pool must be a CUDA tensor (no CPU fallback)");
   const at::Device dev = pool.device();
   c10::cuda::CUDAGuard guard(dev);
   check_opt(pool, dev, "pool", at::kInt);
@@ -430,8 +439,14 @@ TORCH_LIBRARY(nanoserve_b200, m) {
       "Tensor(a!) out, Tensor(b!)? status=None) -> ()");
 }
 
-// CPU pools reach copy_pages too, for its message
-TORCH_LIBRARY_IMPL(nanoserve_b200, CPU, m) { m.impl("copy_pages", &copy_pages_op); }
+// CPU tensors get the ops' own message
+TORCH_LIBRARY_IMPL(nanoserve_b200, CPU, m) {
+  m.impl("process_logits", &process_logits_op);
+  m.impl("process_logits_", &process_logits_into);
+  m.impl("token_logprobs", &token_logprobs_op);
+  m.impl("copy_pages", &copy_pages_op);
+  m.impl("paged_history_gather", &paged_history_gather_op);
+}
 
 // these have no gradient and say so themselves: no autograd layer to go through
 TORCH_LIBRARY_IMPL(nanoserve_b200, Autograd, m) {

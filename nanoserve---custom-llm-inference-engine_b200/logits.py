@@ -71,19 +71,15 @@ def process_logits(
     Bad ids, ranges and indices are skipped and set ``NS_STATUS_*`` bits in
     ``status`` (int32 ``[1]``).  One launch on the current stream of
     ``logits.device``; no synchronisation, graph-capturable."""
-    if logits.dim() != 2:
-        raise ValueError("logits must be [rows, vocab]")
-    if not logits.is_cuda:
-        raise RuntimeError("process_logits needs CUDA logits (no CPU fallback)")
-    if logits.stride(1) != 1 and logits.shape[1] > 1 and out is not logits:
-        logits = logits.contiguous()
-    given = (logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty, presence_penalty,
-             frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows, status)
     if out is None:
-        if out_dtype not in (None, logits.dtype, torch.float32):
-            raise ValueError("out_dtype must be the logits' type or float32")
-        return _process(*given, out_dtype)
+        return _process(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
+                        presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed,
+                        allowed_rows, status, out_dtype)
     if out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out has dtype {out.dtype}, out_dtype is {out_dtype}")
-    _process_into(*given, out)
+    if out is not logits and logits.dim() == 2 and logits.shape[1] > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    _process_into(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
+                  presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows,
+                  status, out)
     return out

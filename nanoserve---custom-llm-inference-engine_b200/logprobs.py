@@ -46,10 +46,4 @@ def token_logprobs(
     outside ``[0, V)`` gets NaN and rank 0, and sets ``NS_STATUS_BAD_TOKEN_ID`` in
     ``status`` (int32 ``[1]``).  One launch on the current stream of
     ``logits.device``; no synchronisation, graph-capturable."""
-    if logits.dim() != 2:
-        raise ValueError("logits must be [rows, vocab]")
-    if not logits.is_cuda:
-        raise RuntimeError("token_logprobs needs CUDA logits (no CPU fallback)")
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
-        logits = logits.contiguous()
-    return TokenLogprobs(*_token_logprobs(logits, sample_indices, token_ids.contiguous(), top_n, status))
+    return TokenLogprobs(*_token_logprobs(logits, sample_indices, token_ids, top_n, status))

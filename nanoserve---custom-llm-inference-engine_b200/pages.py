@@ -59,13 +59,8 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src: Pages, d
     source and a destination.  One launch per 64 pools and 3500 pages on the
     current stream of the pools' device; the page numbers are taken during the
     call, so a graph that captures it replays the same copies."""
-    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     s, d = _page_list(src, "src"), _page_list(dst, "dst")
-    if s.numel() != d.numel():
-        raise ValueError(f"{s.numel()} source pages and {d.numel()} destination pages")
-    if not pools:
-        return
-    _copy_pages(pools, s, d)
+    _copy_pages([pools] if isinstance(pools, torch.Tensor) else pools, s, d)
 
 
 def gather_paged_history(
@@ -87,8 +82,6 @@ def gather_paged_history(
     the status, and rows are left out).  Where a table is too short or a
     page does not exist the id becomes -1 (which the sampler reports) and ``NS_STATUS_BAD_POOL_RANGE`` is
     set in ``status`` (int32 ``[1]``).  One launch on the current stream of ``pool.device``."""
-    if not pool.is_cuda:
-        raise RuntimeError("gather_paged_history needs a CUDA pool (no CPU fallback)")
     _gather(pool, pages, page_offsets, history_offsets, out, status)
     return out
 
