@@ -184,8 +184,8 @@ __device__ __forceinline__ uint32_t widen(uint32_t h) {
 // One tile of one row.  The tile is brought into shared memory by a bulk copy
 // while the block counts the row's history ids that fall into it, 16 bits per id
 // in shared memory, and lists the ids it meets first.  Then each listed id's logit
-// is recomputed where it lies, and the tile leaves through a bulk copy, or, under a
-// mask or with another type, through registers.
+// is recomputed where it lies, what a mask forbids is overwritten, and the tile
+// leaves through a bulk copy (or, with another type, through registers).
 template <typename In, typename Out, bool kInPlace>
 __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
   constexpr bool kSame = sizeof(In) == sizeof(Out);
@@ -346,11 +346,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_co
         else store_f(out + i, -INFINITY);
       }
     } else {
-      if (!mask) {
-        if (tid == 0 && body) bulk_s2g(out + head, x + head, body * sizeof(Out));
-      } else {
+      if (mask) {
+        constexpr uint32_t kAll = (1u << kVec) - 1;
         for (int i = head + tid * kVec; i < head + body; i += kThreads * kVec) {
           const uint32_t bits = mask_bits(mask, mask_words, i);
+          if ((bits & kAll) == kAll) continue;
           uint4 y = *reinterpret_cast<const uint4*>(x + i);
           uint32_t* w = reinterpret_cast<uint32_t*>(&y);
 #pragma unroll
@@ -362,15 +362,18 @@ __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_co
               if (!((bits >> (2 * e + 1)) & 1u)) w[e] = (w[e] & 0xffffu) | 0xff800000u;
             }
           }
-          *reinterpret_cast<uint4*>(out + i) = y;
+          *reinterpret_cast<uint4*>(x + i) = y;
         }
+        fence_proxy_async_smem();
+        __syncthreads();
       }
+      if (tid == 0 && body) bulk_s2g(out + head, x + head, body * sizeof(Out));
       const int e = tid < head ? tid : tid - head < n - head - body ? body + tid : -1;  // the ends
       if (e >= 0) {
         if (allowed(e)) out[e] = x[e];
         else store_f(out + e, -INFINITY);
       }
-      if (!mask && tid == 0) bulk_s2g_wait();  // shared memory is read before the block ends
+      if (tid == 0) bulk_s2g_wait();  // shared memory is read before the block ends
     }
   } else {
     // bf16 in, fp32 out: eight elements at a time from the tile's 16-byte grid
