@@ -154,6 +154,8 @@ struct GatherArgs {
   uint32_t* status;
 };
 
+// kPow2: the page size is a power of two.
+template <bool kPow2>
 __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_constant__ GatherArgs a) {
   __shared__ RowPages s_rows[kThreads / 32][32];
   const int lane = threadIdx.x % 32;
@@ -177,7 +179,9 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
       n = min(step - 1, left);
     }
     const uint32_t size = (uint32_t)a.page_size;
-    const int bits = (size & (size - 1)) == 0 ? 31 - __clz(size) : -1;
+    const int bits = 31 - __clz(size);
+    const uint32_t num_pages = (uint32_t)min(a.num_pages, (int64_t)0x80000000);  // page numbers are 31 bits
+    int32_t* out = a.ids + first + lane;
     RowPages* rows = s_rows[threadIdx.x / 32];
     for (int base = row; base < a.rows; base += 32) {
       const int r = min(base + lane, a.rows - 1);
@@ -210,28 +214,26 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
       }
 #pragma unroll
       for (int k0 = 0; k0 < kEach; k0 += kBatch) {
-        uint32_t rest[kBatch];
-        int id[kBatch];
+        uint32_t rest[kBatch], id[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int pos = (k0 + k) * 32 + lane;
           const RowPages p = rows[at[k0 + k]];
           const uint32_t place = (uint32_t)(pos + p.shift);
-          const uint32_t t = bits >= 0 ? place >> bits : place / size;
-          rest[k] = place - t * size;
-          id[k] = pos >= from && pos < to && t < p.pages ? __ldg(p.list + t) : -1;
+          const uint32_t t = kPow2 ? place >> bits : place / size;
+          rest[k] = kPow2 ? place & (size - 1) : place - t * size;
+          id[k] = pos >= from && pos < to && t < p.pages ? (uint32_t)__ldg(p.list + t) : ~0u;
         }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-          const int64_t page = id[k];
-          if (page >= 0 && page < a.num_pages) id[k] = __ldg(a.pool + (page * size + rest[k]));
-          else id[k] = -1, rest[k] = ~0u;
+          if (id[k] < num_pages) id[k] = (uint32_t)__ldg(a.pool + ((uint64_t)id[k] * size + rest[k]));
+          else id[k] = ~0u, rest[k] = ~0u;
         }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int pos = (k0 + k) * 32 + lane;
           if (pos >= from && pos < to) {
-            a.ids[first + pos] = id[k];
+            out[(k0 + k) * 32] = (int32_t)id[k];
             bad |= rest[k] == ~0u;
           }
         }
@@ -297,7 +299,8 @@ int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page
   if (blocks > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: num_ids is too large");
   const pages::GatherArgs g = {pool, num_pages, page_size, table, num_table_pages, page_offsets, offsets,
                                num_rows, out_ids, num_ids, status};
-  pages::gather_kernel<<<(unsigned)blocks, pages::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(g);
+  const auto kernel = (page_size & (page_size - 1)) == 0 ? pages::gather_kernel<true> : pages::gather_kernel<false>;
+  kernel<<<(unsigned)blocks, pages::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(g);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)
     return fail(NS_ERR_CUDA, std::string("ns_paged_history_gather launch: ") + cudaGetErrorString(e));
