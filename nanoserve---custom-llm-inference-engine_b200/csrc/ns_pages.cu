@@ -121,16 +121,14 @@ std::string check_plan(int64_t num_pages, const int64_t* src, const int64_t* dst
   return wrong;
 }
 
-// out[p] for every position p of the CSR array: a warp owns kChunk consecutive
+// out[p] for every position p of the CSR array: a warp owns kEach * 32 consecutive
 // positions, so that a few long rows and many short ones spread alike.  It finds
 // the row of its first position by a 32-way search of the offsets; then its lanes
 // fetch what 32 rows from there need, one each, and leave it in shared memory, and
 // every lane looks up, for each of its positions (32 apart), its row, the page
 // number and the id.  What is spent is integer work and the latency of that chain
 // of loads: places are 32-bit, and kBatch positions per lane are in flight.
-constexpr int kEach = 8;  // positions per lane
 constexpr int kBatch = 4;
-constexpr int kChunk = kEach * 32;
 
 // A row as its positions in a chunk see it: position pos is place p = pos + shift
 // of the row (counted from the first page that the tables hold), on page
@@ -154,9 +152,10 @@ struct GatherArgs {
   uint32_t* status;
 };
 
-// kPow2: the page size is a power of two.
-template <bool kPow2>
+// kPow2: the page size is a power of two.  kEach: positions per lane.
+template <bool kPow2, int kEach>
 __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_constant__ GatherArgs a) {
+  constexpr int kChunk = kEach * 32;
   __shared__ RowPages s_rows[kThreads / 32][32];
   const int lane = threadIdx.x % 32;
   bool bad = false;
@@ -204,13 +203,12 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
       const int to = (int)max((int64_t)0, min(min(all, end - first), (int64_t)kChunk));
       const int ends = __popc(__ballot_sync(0xffffffffu, e < kChunk) & (uint32_t)((1ull << n) - 1));
       const int e32 = (int)max((int64_t)-1, min(e, (int64_t)kChunk));
-      int at[kEach];
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) at[k] = 0;
+      uint32_t at[kEach / 4] = {};  // a byte per position: which of the window's rows it is in
       for (int k = 0; k < min(ends, n - 1); ++k) {
         const int x = __shfl_sync(0xffffffffu, e32, k);
 #pragma unroll
-        for (int q = 0; q < kEach; ++q) at[q] += x <= q * 32 + lane;
+        for (int q = 0; q < kEach; ++q)
+          if (x <= q * 32 + lane) at[q / 4] += 1u << (q % 4 * 8);
       }
 #pragma unroll
       for (int k0 = 0; k0 < kEach; k0 += kBatch) {
@@ -218,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int pos = (k0 + k) * 32 + lane;
-          const RowPages p = rows[at[k0 + k]];
+          const RowPages p = rows[(at[(k0 + k) / 4] >> ((k0 + k) % 4 * 8)) & 0xffu];
           const uint32_t place = (uint32_t)(pos + p.shift);
           const uint32_t t = kPow2 ? place >> bits : place / size;
           rest[k] = kPow2 ? place & (size - 1) : place - t * size;
@@ -294,12 +292,18 @@ int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page
   if (num_rows == 0 || num_ids == 0) return NS_OK;
   if (!page_offsets || !offsets || !out_ids || (!pool && num_pages > 0) || (!table && num_table_pages > 0))
     return fail(NS_ERR_INVALID_ARG, "ns_paged_history_gather: null device pointer");
-  const int64_t per_block = pages::kChunk * (pages::kThreads / 32);
+  // A warp's search costs as much as several of its positions: sixteen per lane where there are warps enough to
+  // fill the GPU (9.4 M ids: 31 us against 37 with eight), eight where there are not (278 K ids: 5.5 us
+  // against 6.1).
+  const bool many = num_ids >= (int64_t)148 * 48 * 32 * 16;
+  const int64_t per_block = pages::kThreads * (many ? 16 : 8);
   const int64_t blocks = (num_ids + per_block - 1) / per_block;
   if (blocks > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: num_ids is too large");
   const pages::GatherArgs g = {pool, num_pages, page_size, table, num_table_pages, page_offsets, offsets,
                                num_rows, out_ids, num_ids, status};
-  const auto kernel = (page_size & (page_size - 1)) == 0 ? pages::gather_kernel<true> : pages::gather_kernel<false>;
+  const bool pow2 = (page_size & (page_size - 1)) == 0;
+  const auto kernel = many ? (pow2 ? pages::gather_kernel<true, 16> : pages::gather_kernel<false, 16>)
+                           : (pow2 ? pages::gather_kernel<true, 8> : pages::gather_kernel<false, 8>);
   kernel<<<(unsigned)blocks, pages::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(g);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)

@@ -136,7 +136,7 @@ def test_copy_graph_replay_and_streams():
 
 
 @pytest.mark.parametrize("page", [1, 3, 16, 100, 256])
-@pytest.mark.parametrize("rows,hi", [(1, 1), (7, 40), (300, 900), (3, 50000)])
+@pytest.mark.parametrize("rows,hi", [(1, 1), (7, 40), (300, 900), (3, 50000), (9000, 900)])
 def test_gather_equals_indexing(page, rows, hi):
     rng = np.random.default_rng(page + rows)
     lens = rng.integers(0, hi + 1, rows)
