@@ -433,13 +433,13 @@ struct Table {
 // addressing, at most half full) and recomputes each once.  Rows with more ids
 // than the table takes are left to the kHelpers blocks behind: every one finds
 // these rows, and they share out their ranges of kRange ids, one word per id.
-constexpr int kSparseThreads = 1024;
+constexpr int kSparseThreads = 512;
 constexpr int kRowSlots = 8192;  // most slots of a row's table, a power of two
 constexpr int kRange = 2 * kRowSlots;
 constexpr int kHelpers = 32;
 
 template <typename T>
-__global__ void __launch_bounds__(kSparseThreads) sparse_kernel(const __grid_constant__ NsProcessArgs a) {
+__global__ void __launch_bounds__(kSparseThreads, 2) sparse_kernel(const __grid_constant__ NsProcessArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   uint32_t* words = reinterpret_cast<uint32_t*>(smem);  // kRowSlots words and as many ids, or kRange words
   uint32_t* ids = words + kRowSlots;
