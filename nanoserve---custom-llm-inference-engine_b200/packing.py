@@ -211,8 +211,9 @@ EXTENDED_FIELDS = ("presence_penalty", "frequency_penalty", "logit_bias")
 def wants_processing(params: Sequence) -> bool:
     """Whether some request carries a presence or frequency penalty or a bias.
     Looks at the requests only if one of their types has these fields."""
-    types = {type(p): p for p in params}
-    if not any(hasattr(p, f) for p in types.values() for f in EXTENDED_FIELDS):
+    kinds = set(map(type, params))
+    one_of_each = params[:1] if len(kinds) == 1 else {type(p): p for p in params}.values()
+    if not any(hasattr(p, f) for p in one_of_each for f in EXTENDED_FIELDS):
         return False
     return any(getattr(p, f, None) for p in params for f in EXTENDED_FIELDS)
 
