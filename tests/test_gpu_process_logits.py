@@ -160,17 +160,23 @@ def test_strided_and_unaligned_rows(dtype, offset):
     _check(NS.process_logits(x[:S].t().contiguous().t(), **kw), x[:S].double().cpu().numpy(), d, dtype)
 
 
-@pytest.mark.parametrize("in_place", [False, True])
-def test_long_repetitive_histories(in_place):
-    """Counts of many thousands, ids that share a bank, histories longer than the vocabulary."""
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("types", TYPES + [(torch.float32, None), (torch.bfloat16, None)],
+                         ids=["f32", "bf16-f32", "bf16", "f32-in-place", "bf16-in-place"])
+def test_long_repetitive_histories(types, mask):
+    """Counts of many thousands, neighbouring ids of which one has many, histories longer than the vocabulary, and
+    more different ids than a block lists."""
     rng = np.random.default_rng(9)
-    S, V = 3, 40000
-    hists = [[17] * 30000 + [39999] * 5, rng.integers(0, V, 131072).tolist(), (np.arange(60000) * 32 % V).tolist()]
-    d = dict(hists=hists, prompts=[10, 70000, 0], rep=[1.2, 1.1, 1.0], pres=[0.1, 0.2, 0.3], freq=[0.01, 0.5, 0.25],
-             biases=[[], [(5, 1.0)], []], masks=None)
-    x = torch.from_numpy(rng.normal(0, 3, (S, V)).astype(np.float32)).to(_dev())
+    S, V = 4, 40000
+    hists = [[17] * 30000 + [39999] * 5 + [16, 18], rng.integers(0, V, 131072).tolist(), (np.arange(60000) * 32 % V).tolist(),
+             [20000] * 6990 + [20001] * 7100 + rng.integers(0, 9000, 5000).tolist()]
+    d = dict(hists=hists, prompts=[10, 70000, 0, 4], rep=[1.2, 1.1, 1.0, 1.3], pres=[0.1, 0.2, 0.3, 0.4],
+             freq=[0.01, 0.5, 0.25, 0.125], biases=[[(16, 2.0)], [(5, 1.0)], [], [(20001, -1.0), (20001, 4.0), (30000, 1.0)]],
+             masks=[rng.random(V) < 0.5 for _ in range(S)] if mask else None)
+    x = torch.from_numpy(rng.normal(0, 3, (S, V)).astype(np.float32)).to(_dev()).to(types[0])
     rows = x.double().cpu().numpy()
-    _check(NS.process_logits(x, out=x if in_place else None, **_device(d, V)), rows, d, torch.float32)
+    got = NS.process_logits(x, out=x if types[1] is None else None, out_dtype=types[1], **_device(d, V))
+    _check(got, rows, d, types[1] or types[0])
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
