@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "ns_device.cuh"
 
@@ -30,7 +31,6 @@ namespace lp {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
 constexpr int kMaxCluster = 8;     // the portable limit
 constexpr float kLag = 8.0f;       // the reference follows the maximum in steps of at least this
 constexpr float kHuge = 0x1p100f;  // beyond it the fused argument of the exponential could overflow
@@ -76,6 +76,7 @@ struct Row;
 template <>
 struct Row<float> {
   static constexpr int kVec = 4;
+  static constexpr int kUnroll = 6;  // 16-byte loads in flight per thread
   __device__ static float one(const float* p) { return __ldg(p); }
   struct Vec {
     float4 v;
@@ -107,6 +108,7 @@ struct Row<float> {
 template <>
 struct Row<__nv_bfloat16> {
   static constexpr int kVec = 8;
+  static constexpr int kUnroll = 8;
   __device__ static float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   struct Vec {
     uint32_t w[4];
@@ -230,7 +232,7 @@ template <typename In>
 __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArgs a, int C) {
   using R = Row<In>;
   using Vec = typename R::Vec;
-  constexpr int kVec = R::kVec;
+  constexpr int kVec = R::kVec, kUnroll = R::kUnroll;
   __shared__ float s_max[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_cnt[kWarps];
@@ -289,26 +291,26 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
     }
   };
   int i = lo + tid;
-  for (; i + (kUnroll - 1) * kThreads < hi; i += kUnroll * kThreads) {
-    Vec b[kUnroll];
+  const auto take = [&](auto size) {  // the next vectors of the bucket, that many at once; their maximum
+    constexpr int N = decltype(size)::value;
+    Vec b[N];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) b[u].load(xv + (int64_t)(i + u * kThreads) * kVec);
+    for (int u = 0; u < N; ++u) b[u].load(xv + (int64_t)(i + u * kThreads) * kVec);
+    i += N * kThreads;
     const float bm = R::max_of(b);
-    m = fmax_nan(m, bm);
-    if (n > 1) note(bm);
     count.add(b);
     sum.template add<R>(b, bm);
+    return bm;
+  };
+  while (i + (kUnroll - 1) * kThreads < hi) {
+    const float bm = take(std::integral_constant<int, kUnroll>{});
+    m = fmax_nan(m, bm);
+    if (n > 1) note(bm);
   }
   float rest = -INFINITY;
   const bool some = i < hi;
-  for (; i < hi; i += kThreads) {
-    Vec b[1];
-    b[0].load(xv + (int64_t)i * kVec);
-    const float bm = R::max_of(b);
-    rest = fmax_nan(rest, bm);
-    count.add(b);
-    sum.template add<R>(b, bm);
-  }
+  if (i + (kUnroll / 2 - 1) * kThreads < hi) rest = take(std::integral_constant<int, kUnroll / 2>{});
+  while (i < hi) rest = fmax_nan(rest, take(std::integral_constant<int, 1>{}));
   m = fmax_nan(m, rest);
   if (n == 1 && lo + tid < hi) {
     entry = f2key(m + 0.0f);
