@@ -342,6 +342,14 @@ int ns_token_logprobs(const NsLogprobArgs* args, void* stream);
  * twice, or a page that is both source and destination is refused
  * (NS_ERR_INVALID_ARG) before anything is enqueued.
  *
+ * ns_pages_check: ns_pages_copy's check of the page numbers alone (host only).
+ *
+ * ns_pages_copy_listed: the same copies with src and dst in DEVICE memory (one
+ * launch for any count, where ns_pages_copy takes one per 3500).  A page
+ * outside [0, num_pages) is skipped and sets NS_STATUS_BAD_POOL_RANGE; the
+ * rest of the rules is the caller's (where they are broken, the pages named
+ * get the bytes of some of the sources).
+ *
  * ns_paged_history_gather: row r's prior ids out of a pool of int32 pages,
  *   out_ids[offsets[r] + j] = pool[pages[page_offsets[r] + j / page_size] * page_size + j % page_size]
  *   for j < offsets[r+1] - offsets[r]: the CSR history_ids of NsSampleArgs
@@ -359,6 +367,9 @@ typedef struct NsPagePool {
 
 int ns_pages_copy(const NsPagePool* pools, int32_t num_pools, int64_t num_pages, const int64_t* src,
                   const int64_t* dst, int64_t count, void* stream);
+int ns_pages_check(int64_t num_pages, const int64_t* src, const int64_t* dst, int64_t count);
+int ns_pages_copy_listed(const NsPagePool* pools, int32_t num_pools, int64_t num_pages, const int32_t* src,
+                         const int32_t* dst, int64_t count, uint32_t* status, void* stream);
 int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page_size, const int32_t* pages,
                             int64_t num_table_pages, const int64_t* page_offsets, const int64_t* offsets,
                             int32_t num_rows, int32_t* out_ids, int64_t num_ids, uint32_t* status, void* stream);

@@ -49,6 +49,7 @@ NS_MAX_TOP_LOGPROBS = 32
 # every entry point the header declares
 EXPORTED_SYMBOLS = ("ns_sample", "ns_sample_noalloc", "ns_workspace_bytes", "ns_history_gather",
                     "ns_history_append", "ns_process_logits", "ns_token_logprobs", "ns_pages_copy",
+                    "ns_pages_check", "ns_pages_copy_listed",
                     "ns_paged_history_gather", "ns_last_error", "ns_abi_version", "ns_max_vocab")
 NS_ABI_VERSION = 3
 NS_NOALLOC_WORKSPACE_BYTES = 128
@@ -194,6 +195,13 @@ def load_library() -> ctypes.CDLL:
                                       ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),
                                       ctypes.c_int64, ctypes.c_void_p]
         lib.ns_pages_copy.restype = ctypes.c_int
+        lib.ns_pages_check.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_int64),
+                                       ctypes.POINTER(ctypes.c_int64), ctypes.c_int64]
+        lib.ns_pages_check.restype = ctypes.c_int
+        lib.ns_pages_copy_listed.argtypes = [ctypes.POINTER(NsPagePool), ctypes.c_int32, ctypes.c_int64,
+                                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                             ctypes.c_void_p]
+        lib.ns_pages_copy_listed.restype = ctypes.c_int
         lib.ns_paged_history_gather.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
                                                 ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
                                                 ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]
@@ -282,6 +290,22 @@ def ns_pages_copy(pools: Sequence, num_pages: int, src: Sequence[int], dst: Sequ
     n = len(src)
     ids = ctypes.c_int64 * max(1, n)
     _call("ns_pages_copy", p, len(pools), num_pages, ids(*src), ids(*dst), n, ctypes.c_void_p(stream))
+
+
+def ns_pages_check(num_pages: int, src: Sequence[int], dst: Sequence[int]) -> None:
+    """The check of the page numbers that ``ns_pages_copy`` makes."""
+    if len(src) != len(dst):
+        raise ValueError("src and dst must have the same number of pages")
+    ids = ctypes.c_int64 * max(1, len(src))
+    _call("ns_pages_check", num_pages, ids(*src), ids(*dst), len(src))
+
+
+def ns_pages_copy_listed(pools: Sequence, num_pages: int, src: int, dst: int, count: int, status: int = 0,
+                         stream: int = 0) -> None:
+    """``ns_pages_copy`` with the page numbers in device memory (int32, device pointers as ints)."""
+    p = (NsPagePool * max(1, len(pools)))(*[x if isinstance(x, NsPagePool) else NsPagePool(*x) for x in pools])
+    _call("ns_pages_copy_listed", p, len(pools), num_pages, src or None, dst or None, count, status or None,
+          ctypes.c_void_p(stream))
 
 
 def ns_paged_history_gather(pool: int, num_pages: int, page_size: int, pages: int, num_table_pages: int,

@@ -15,6 +15,14 @@
 // the elements that reach the bound are ranked by counting (or, where ties make
 // them many, through sorted lists), within the block and then, through
 // distributed shared memory, within the cluster.
+//
+// Measured on a B200 (V = 128256; the logits' bytes at the 6446 GB/s of a copy in
+// brackets): 4096 bf16 rows, top 1: 175 us (163); 256 fp32 rows, top 20: 33 us
+// (20); 8 fp32 rows, top 5: 10 us (0.6).  Large batches are bound by the loads,
+// with the exponential units two thirds busy; a few hundred rows are one wave of
+// blocks, whose search for the top tokens (about 6 us after the 20 us of loads)
+// nothing overlaps: four blocks a row in place of two took 42 us, as each block
+// pays for its own.  Eight rows are bound by the launch and the chain of barriers.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -500,6 +508,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
 
 template <typename In>
 cudaError_t launch(const NsLogprobArgs& a, cudaStream_t st) {
+  // Blocks per row: as many as bring about two per SM onto the GPU.  (Top 20 in us with 1, 2, 4 blocks: 256 fp32
+  // rows 42, 33, 42; 1024 bf16 rows 64, 83, 115; with 2, 4, 8: 64 fp32 rows 26, 21, 21, 8 rows 18, 15, 13.5.)
   int C = 1;
   while (C < kMaxCluster && (int64_t)a.num_rows * C < 148 * 2 && a.vocab_size / C >= 4096) C *= 2;
   cudaLaunchConfig_t cfg = {};

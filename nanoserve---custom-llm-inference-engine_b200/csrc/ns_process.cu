@@ -186,6 +186,16 @@ __device__ __forceinline__ uint32_t widen(uint32_t h) {
 // in shared memory, and lists the ids it meets first.  Then each listed id's logit
 // is recomputed where it lies, what a mask forbids is overwritten, and the tile
 // leaves through a bulk copy (or, with another type, through registers).
+//
+// 256 rows of 128256 fp32 with histories of about 1088 take 45 us (263.9 MB at the
+// 6446 GB/s of a copy: 41), without histories 43; 2048 rows of 50257 under masks
+// 157 us (130); 64 bf16 rows into fp32 under masks, histories of about 2300, 22 to 24
+// us (8).  Bulk copies need no registers and few instructions; what is left is a
+// block's chain of dependent loads (offsets, ids, the tile) and barriers, about 6 us
+// during which three blocks have 144 KB on their way on each SM.  Reading and writing
+// through registers, with the named ids corrected in global memory afterwards, took
+// 88 us (histories) and 51 us (none): the corrections are partial writes to lines
+// that are on their way out.  A hash table in place of 16 bits per id took 53 us.
 template <typename In, typename Out, bool kInPlace>
 __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
   constexpr bool kSame = sizeof(In) == sizeof(Out);
@@ -433,6 +443,11 @@ struct Table {
 // addressing, at most half full) and recomputes each once.  Rows with more ids
 // than the table takes are left to the kHelpers blocks behind: every one finds
 // these rows, and they share out their ranges of kRange ids, one word per id.
+//
+// 256 rows of 128256 fp32 with histories of about 1088 ids take 20 us, all rows'
+// blocks resident at once: about half is the 278 thousand scattered reads and
+// writes of logits (a run without them took 8 to 11), the rest the longest rows' chain
+// of table accesses.
 constexpr int kSparseThreads = 512;
 constexpr int kRowSlots = 8192;  // most slots of a row's table, a power of two
 constexpr int kRange = 2 * kRowSlots;

@@ -345,6 +345,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_op(
   return result;
 }
 
+constexpr int64_t kLongList = 3500;  // what ns_pages_copy takes in one launch
+
 // copy_pages(pools, src, dst) -> (): src and dst are CPU int64 lists of pages
 void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor& dst) {
   TORCH_CHECK(src.device().is_cpu() && dst.device().is_cpu() && src.scalar_type() == at::kLong &&
@@ -378,9 +380,27 @@ void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor
     return;
   }
   c10::cuda::CUDAGuard guard(dev);
-  const int rc = ns_pages_copy(p.data(), (int32_t)p.size(), num_pages, static_cast<const int64_t*>(src.data_ptr()),
-                               static_cast<const int64_t*>(dst.data_ptr()), src.numel(),
-                               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  const int64_t n = src.numel();
+  const int64_t *s = static_cast<const int64_t*>(src.data_ptr()), *d = static_cast<const int64_t*>(dst.data_ptr());
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (n > kLongList)
+    TORCH_CHECK(cudaStreamIsCapturing(stream, &cap) == cudaSuccess, "cudaStreamIsCapturing failed");
+  int rc;
+  if (n > kLongList && cap == cudaStreamCaptureStatusNone && num_pages <= INT32_MAX) {
+    rc = ns_pages_check(num_pages, s, d, n);
+    if (rc == NS_OK) {
+      // one copy of the lists (both allocators keep what is in flight) in place of a launch for each few thousand
+      const at::Tensor host = at::empty({2, n}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+      host[0].copy_(src.view({n}));
+      host[1].copy_(dst.view({n}));
+      const at::Tensor lists = host.to(dev, /*non_blocking=*/true);
+      const int32_t* l = static_cast<const int32_t*>(lists.data_ptr());
+      rc = ns_pages_copy_listed(p.data(), (int32_t)p.size(), num_pages, l, l + n, n, nullptr, stream);
+    }
+  } else {
+    rc = ns_pages_copy(p.data(), (int32_t)p.size(), num_pages, s, d, n, stream);
+  }
   TORCH_CHECK_VALUE(rc != NS_ERR_INVALID_ARG, ns_last_error());
   TORCH_CHECK(rc == NS_OK, "ns_pages_copy failed (", rc, "): ", ns_last_error());
 }

@@ -56,9 +56,10 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src: Pages, d
     ``src`` and ``dst`` are lists, arrays or CPU tensors of page numbers.  A page
     may be copied to several places; ``ValueError`` is raised, and nothing
     copied, where a page does not exist, is a destination twice, or is both a
-    source and a destination.  One launch per 64 pools and 3500 pages on the
-    current stream of the pools' device; the page numbers are taken during the
-    call, so a graph that captures it replays the same copies."""
+    source and a destination.  One launch per 64 pools on the current stream of
+    the pools' device (lists of more than 3500 pages are uploaded first, or, in a
+    stream capture, take a launch per 3500); the page numbers are taken during
+    the call, so a graph that captures it replays the same copies."""
     s, d = _page_list(src, "src"), _page_list(dst, "dst")
     _copy_pages([pools] if isinstance(pools, torch.Tensor) else pools, s, d)
 
@@ -269,8 +270,7 @@ class PagedHistoryStore(StoreSampling):
         self._alloc.free(self._requests.pop(handle).pages)
 
     def compact(self) -> int:
-        """Move the live pages to the front of the pool and of the caches (one launch per 3500
-        moves); returns how many moved.  Page tables taken before are stale."""
+        """Move the live pages to the front of the pool and of the caches; returns how many moved.  Page tables taken before are stale."""
         src, dst = self._alloc.plan_compact()
         if src.size:
             copy_pages([self.pool, *self.caches], src, dst)

@@ -93,6 +93,43 @@ def test_pools_past_2_to_the_31_bytes():
     assert (p[n - 2] == 7).all() and (p[6] == 9).all() and not p[7].any() and not p[n - 3].any()
 
 
+def test_listed_copies():
+    """Page numbers in device memory: one launch, pages outside the pool skipped and reported."""
+    p = _bits((9000, 16), torch.int32, 3)
+    order = np.random.default_rng(2).permutation(9000)
+    src, dst = order[:4400], order[4400:8800]
+    want = _copied([p], src, dst)[0]
+    bad = [(9000, int(order[8900])), (-1, int(order[8901])), (int(order[8902]), 9000), (int(order[8903]), -7)]
+    s = torch.tensor([*src.tolist(), *[a for a, _ in bad]], dtype=torch.int32, device=_dev())
+    d = torch.tensor([*dst.tolist(), *[b for _, b in bad]], dtype=torch.int32, device=_dev())
+    st = torch.zeros(1, dtype=torch.int32, device=_dev())
+    pool = [(p.data_ptr(), 64, 64)]
+    stream = torch.cuda.current_stream().cuda_stream
+    cabi.ns_pages_copy_listed(pool, 9000, s.data_ptr(), d.data_ptr(), 4400, st.data_ptr(), stream)
+    assert st.item() == 0 and torch.equal(p, want)
+    cabi.ns_pages_copy_listed(pool, 9000, s.data_ptr(), d.data_ptr(), 4404, st.data_ptr(), stream)
+    assert st.item() == cabi.NS_STATUS_BAD_POOL_RANGE and torch.equal(p, want)
+
+
+def test_long_lists_in_a_graph():
+    """More pages than a launch takes, captured: the page numbers become part of the graph."""
+    p = _bits((20000, 16), torch.int32, 3)
+    order = torch.randperm(20000)
+    src, dst = order[:8000].clone(), order[8000:16000].clone()
+    NS.copy_pages(p, [0], [1])
+    g = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=side):
+        NS.copy_pages(p, src, dst)
+    p.copy_(_bits((20000, 16), torch.int32, 4))
+    want = _copied([p], src, dst)[0]
+    src.zero_(), dst.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p, want)
+
+
 def test_copy_refusals_leave_the_pools():
     p = _bits((8, 16), torch.int32, 1)
     was = p.clone()

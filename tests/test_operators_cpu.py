@@ -84,6 +84,46 @@ def test_page_copies_are_checked_on_the_host(pool, pages_n, src, dst, match):
         cabi.ns_pages_copy([pool], pages_n, src, dst)
 
 
+def test_page_checks_on_long_lists():
+    """Random plans with one thing wrong somewhere, among sound ones; a refusal leaves nothing behind."""
+    rng = random.Random(4)
+    for n, pages_n in ((1, 2), (5, 40), (300, 1000), (4000, 9000), (500, 100000)):
+        for _ in range(6):
+            order = rng.sample(range(pages_n), 2 * n)
+            src, dst = order[:n], order[n:]
+            cabi.ns_pages_check(pages_n, src, dst)
+            cabi.ns_pages_check(pages_n, [src[0]] * n, dst)
+            low, high = sorted(order)[:n], sorted(order)[n:]
+            cabi.ns_pages_check(pages_n, high, low)  # as a compaction's
+            cabi.ns_pages_check(pages_n, low, high)
+            i, j = rng.randrange(n), rng.randrange(n)
+            for bad, match in ((-1, "outside"), (pages_n, "outside"), (1 << 62, "outside"), (src[j], "both")):
+                with pytest.raises(cabi.NsError, match=match):
+                    cabi.ns_pages_check(pages_n, src, dst[:i] + [bad] + dst[i + 1:])
+            for bad, match in ((-5, "outside"), (pages_n, "outside"), (dst[j], "both")):
+                with pytest.raises(cabi.NsError, match=match):
+                    cabi.ns_pages_check(pages_n, src[:i] + [bad] + src[i + 1:], dst)
+            if n > 1 and i != j:
+                with pytest.raises(cabi.NsError, match="twice"):
+                    cabi.ns_pages_check(pages_n, src, dst[:i] + [dst[j]] + dst[i + 1:])
+                with pytest.raises(cabi.NsError, match="twice"):
+                    cabi.ns_pages_check(pages_n, high, [low[max(k, 1) - 1] if k == max(i, 1) else x for k, x in enumerate(low)])
+                with pytest.raises(cabi.NsError, match="outside"):
+                    cabi.ns_pages_check(pages_n, high[:-1] + [pages_n + 3], low)
+    with pytest.raises(cabi.NsError, match="null"):
+        cabi._call("ns_pages_check", 5, None, None, 2)
+    with pytest.raises(cabi.NsError, match="< 0"):
+        cabi.ns_pages_check(-1, [0], [1])
+
+
+def test_listed_copies_are_checked_on_the_host():
+    for args, match in ((([(64, 16, 16)], 4, 0, 16, 1), "null"), (([(64, 8, 16)], 4, 16, 16, 1), "overlap"),
+                        (([(64, 16, 16)], 4, 16, 16, -1), "< 0"), (([(64, 16, 16)], 1 << 31, 16, 16, 1), "2\\^31")):
+        with pytest.raises(cabi.NsError, match=match):
+            cabi.ns_pages_copy_listed(*args)
+    cabi.ns_pages_copy_listed([], 0, 0, 0, 0)
+
+
 def test_gather_is_checked_on_the_host():
     for args, match in (((16, 4, 0, 16, 4, 16, 16, 1, 16, 4), "page_size"), ((16, -1, 4, 16, 4, 16, 16, 1, 16, 4), "< 0"),
                         ((16, 4, 4, 16, 4, 0, 16, 1, 16, 4), "null"), ((0, 4, 4, 16, 4, 16, 16, 1, 16, 4), "null"),
