@@ -48,10 +48,11 @@ constexpr int kCands = 256;        // candidates that are ranked by counting
 typedef unsigned long long u64;
 static_assert(kMaxCluster * NS_MAX_TOP_LOGPROBS <= kThreads, "every thread ranks one key of the cluster's");
 
-// Larger value first, then smaller id, as one key to maximise; -0 counts as 0.
-// No logit's key is 0.
+// Larger value first, then smaller id, as one key to maximise; -0 counts as 0, and
+// masked elements (-inf) have key 0: they are the last to be taken, by id.
+__device__ __forceinline__ uint32_t value_key(float x) { return x == -INFINITY ? 0u : f2key(x + 0.0f); }
 __device__ __forceinline__ u64 top_key(float x, int v) {
-  return ((u64)f2key(x + 0.0f) << 32) | (uint32_t)~v;
+  return x == -INFINITY ? 0ull : ((u64)f2key(x + 0.0f) << 32) | (uint32_t)~v;
 }
 __device__ __forceinline__ int top_id(u64 k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float top_value(u64 k) { return key2f((uint32_t)(k >> 32)); }
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   __shared__ double s_sum[kWarps];
   __shared__ int s_cnt[kWarps];
   __shared__ uint32_t s_entry[kEntries][kThreads];
-  __shared__ uint32_t s_few[kWarps];
+  __shared__ uint32_t s_few[kWarps], s_bound;
   __shared__ uint16_t s_list[kListed];
   __shared__ int s_listed, s_cands;
   __shared__ u64 s_best[kThreads];  // sorted keys: the warps', then the block's, then the row's
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   uint32_t bucket = 0, entry = 0;  // keys of maxima: this thread's, and the current entry's (0: nothing)
   int entries = 0, in_entry = 0;
   const auto note = [&](float bm) {
-    entry = max(entry, f2key(bm + 0.0f));
+    entry = max(entry, value_key(bm));
     if (++in_entry == group) {
       s_entry[entries++][tid] = entry;
       bucket = max(bucket, entry);
@@ -321,12 +322,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   while (i < hi) rest = fmax_nan(rest, take(std::integral_constant<int, 1>{}));
   m = fmax_nan(m, rest);
   if (n == 1 && lo + tid < hi) {
-    entry = f2key(m + 0.0f);
+    entry = value_key(m);
   } else if (n > 1 && some) {
-    entry = max(entry, f2key(rest + 0.0f));
+    entry = max(entry, value_key(rest));
   }
   if (n > 0) {
-    if (entry) s_entry[entries++][tid] = entry;
+    if (entry) s_entry[entries++][tid] = entry;  // (one without a key is behind all others)
     bucket = max(bucket, entry);
   }
   int cnt = count.total();
@@ -371,9 +372,21 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
     uint32_t bound = s_few[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) bound = n == 1 ? max(bound, s_few[w]) : min(bound, s_few[w]);
+    if (n > 1 && bound == 0) {
+      // A warp has fewer buckets with anything in them than it should: the n-th largest of all buckets (0 if there
+      // are fewer).
+      s_best[tid] = bucket;
+      if (tid == 0) s_bound = 0;
+      __syncthreads();
+      int more = 0, same = 0;
+      for (int j = 0; j < kThreads; ++j) more += s_best[j] > bucket, same += s_best[j] == bucket;
+      if (more < n && n <= more + same) s_bound = bucket;  // one value, whoever writes it
+      __syncthreads();
+      bound = s_bound;
+    }
     if (bucket && bucket >= bound)
       for (int e = 0; e < entries; ++e)
-        if (s_entry[e][tid] >= bound) {
+        if (s_entry[e][tid] && s_entry[e][tid] >= bound) {
           const int k = atomicAdd(&s_listed, 1);
           if (k < kListed) s_list[k] = (uint16_t)(e * kThreads + tid);
         }
@@ -390,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
         y.load(xv + (int64_t)j * kVec);
 #pragma unroll
         for (int k = 0; k < kVec; ++k)
-          if (y.get(k) >= least) {
+          if (y.get(k) >= least && y.get(k) > -INFINITY) {
             const int c = atomicAdd(&s_cands, 1);
             if (c < kCands) s_cand[c] = top_key(y.get(k), head + j * kVec + k);
           }
@@ -497,12 +510,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
     a.out_ranks[row] = !tok_ok ? 0 : uniform ? 1 : 1 + p.count;
     if (bad && a.status) atomicOr(a.status, bad);
   }
+  // Where fewer than n tokens are not masked, the masked ones follow by id: among the first 64 ids (or all)
+  // there are enough of them.
+  const int found = __popc(__ballot_sync(0xffffffffu, list != 0));
+  int masked = 0;
+  if (found < n && !uniform) {
+    const uint32_t m0 = __ballot_sync(0xffffffffu, lane < V && R::one(x + lane) == -INFINITY);
+    const uint32_t m1 = __ballot_sync(0xffffffffu, lane + 32 < V && R::one(x + lane + 32) == -INFINITY);
+    const int k = lane - found + 1;  // the k-th masked id
+    masked = k <= __popc(m0) ? (int)__fns(m0, 0, max(k, 1)) : 32 + (int)__fns(m1, 0, k - __popc(m0));
+  }
   if (lane < n) {
     const int64_t at = (int64_t)row * n + lane;
-    const int id = uniform ? lane : top_id(list);
+    const int id = uniform ? lane : list ? top_id(list) : masked;
     if (a.ids_dtype == NS_OUT_I64) static_cast<int64_t*>(a.out_top_ids)[at] = id;
     else static_cast<int32_t*>(a.out_top_ids)[at] = id;
-    a.out_top_logprobs[at] = uniform ? -logsum : (top_value(list) - top) - logsum;
+    a.out_top_logprobs[at] = uniform ? -logsum : list ? (top_value(list) - top) - logsum : -INFINITY;
   }
 }
 

@@ -186,6 +186,7 @@ class PagedHistoryStore(StoreSampling):
                 raise ValueError(f"a cache of shape {tuple(c.shape)} does not have {self.num_pages} pages")
         self.pool = torch.zeros(self.num_pages, self.page_size, dtype=torch.int32, device=self.device)
         self.device = self.pool.device
+        copy_pages([self.pool, *self.caches], [], [])  # refuses caches that cannot be copied with the pool
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._alloc = PageAllocator(self.num_pages)
         self._requests: Dict[int, _Request] = {}
@@ -232,7 +233,8 @@ class PagedHistoryStore(StoreSampling):
         full, rest = divmod(r.length, self.page_size)
         own = self._alloc.alloc(n if rest else 0)
         if own:
-            copy_pages([self.pool, *self.caches], [r.pages[full]] * n, own)
+            with torch.cuda.device(self.device):
+                copy_pages([self.pool, *self.caches], [r.pages[full]] * n, own)
         out = []
         for i in range(n):
             self._alloc.share(r.pages[:full])
@@ -260,7 +262,8 @@ class PagedHistoryStore(StoreSampling):
                 mine = self._alloc.alloc(1)[0]
             else:
                 gone.remove(mine)
-            copy_pages([self.pool, *self.caches], [kept[-1]], [mine])
+            with torch.cuda.device(self.device):
+                copy_pages([self.pool, *self.caches], [kept[-1]], [mine])
             gone.append(kept[-1])
             kept[-1] = mine
         self._alloc.free(gone)
@@ -273,7 +276,8 @@ class PagedHistoryStore(StoreSampling):
         """Move the live pages to the front of the pool and of the caches; returns how many moved.  Page tables taken before are stale."""
         src, dst = self._alloc.plan_compact()
         if src.size:
-            copy_pages([self.pool, *self.caches], src, dst)
+            with torch.cuda.device(self.device):
+                copy_pages([self.pool, *self.caches], src, dst)
             to = np.arange(self.num_pages)
             to[src] = dst
             for r in self._requests.values():
@@ -313,6 +317,22 @@ class PagedHistoryStore(StoreSampling):
     def _history_ids(self, parts: Sequence[torch.Tensor], offsets: torch.Tensor, ids: torch.Tensor) -> None:
         gather_paged_history(self.pool, parts[1], parts[0], offsets, out=ids, status=self.status)
 
+    def _grow(self, handles: Sequence[int]) -> None:
+        """A page for the next token of each of these requests (all of them, or MemoryError and none)."""
+        if len(set(handles)) != len(handles):
+            raise ValueError("a request appears twice")
+        grow = [r for r in (self._requests[h] for h in handles) if r.length == len(r.pages) * self.page_size]
+        for r, p in zip(grow, self._alloc.alloc(len(grow))):
+            r.pages.append(p)
+
+    def sample(self, sampler: Sampler, logits: torch.Tensor, sampling_params_list: Sequence, handles: Sequence[int],
+               *, append: bool = True, **kw):
+        if append:
+            self._grow(handles)  # a full pool is found out before anything is sampled
+        return super().sample(sampler, logits, sampling_params_list, handles, append=append, **kw)
+
+    sample.__doc__ = StoreSampling.sample.__doc__
+
     def append(self, handles: Sequence[int], tokens: torch.Tensor) -> None:
         """Append ``tokens[i]`` (device int64 or int32 [S]) to request ``handles[i]``."""
         S = len(handles)
@@ -320,12 +340,8 @@ class PagedHistoryStore(StoreSampling):
             raise ValueError("tokens must be a device tensor with one id per handle")
         if tokens.dtype not in (torch.int64, torch.int32):
             raise ValueError("tokens must be int64 or int32")
-        if len(set(handles)) != S:
-            raise ValueError("a request appears twice")
+        self._grow(handles)
         reqs = [self._requests[h] for h in handles]
-        grow = [r for r in reqs if r.length == len(r.pages) * self.page_size]
-        for r, p in zip(grow, self._alloc.alloc(len(grow))):
-            r.pages.append(p)
         dst = np.fromiter((r.pages[r.length // self.page_size] * self.page_size + r.length % self.page_size
                            for r in reqs), dtype=np.int64, count=S)
         with torch.cuda.device(self.device):

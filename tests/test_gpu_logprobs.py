@@ -104,6 +104,23 @@ def test_masked_and_degenerate_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 2, 5, 31, 33, 63, 64, 65, 100, 700, 20000])
+def test_more_top_tokens_than_are_allowed(V, dtype):
+    """Rows of few allowed tokens, anywhere in the row: the masked ones follow by id."""
+    rng = np.random.default_rng(V)
+    S, n = 24, min(V, 32)
+    x = rng.normal(0, 3, (S, V)).astype(np.float32)
+    for i in range(S):
+        keep = rng.choice(V, min(V, int(rng.integers(0, 40))), replace=False) if i else np.arange(min(V, 31))
+        mask = np.ones(V, dtype=bool)
+        mask[keep] = False
+        x[i, mask] = -np.inf
+    x = torch.from_numpy(x).to(_dev()).to(dtype)
+    t = rng.integers(0, V, S)
+    _check(NS.token_logprobs(x, torch.from_numpy(t).to(_dev()), n), x.double().cpu().numpy(), t, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("offset", [0, 1, 5])
 def test_strided_rows_and_sample_indices(dtype, offset):
     rng = np.random.default_rng(offset)

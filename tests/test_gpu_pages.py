@@ -347,6 +347,29 @@ def test_store_refusals_change_nothing():
     assert st.tokens(a) == [*range(10), 55] and st.tokens(b) == [0, 1, 2, 3, 4, 5, 77, 66]
 
 
+def test_store_refuses_caches_it_cannot_copy():
+    ok = torch.zeros(8, 2, 3, device=_dev())
+    for bad in (torch.zeros(7, 2, device=_dev()), torch.zeros(8, 2), torch.zeros(8, 3, 2, device=_dev()).transpose(1, 2),
+                torch.zeros((), device=_dev())):
+        with pytest.raises((ValueError, RuntimeError)):
+            NS.PagedHistoryStore(_dev(), 8, 10, 4, caches=[ok, bad])
+    NS.PagedHistoryStore(_dev(), 8, 10, 4, caches=[ok])
+
+
+def test_a_full_pool_is_found_out_before_sampling():
+    st = _store(pages=3, page_size=2, vocab=50)
+    a, b = st.add([1, 2]), st.add([3, 4])
+    s = NS.Sampler(_dev())
+    lg = torch.randn(2, 50, device=_dev())
+    with pytest.raises(MemoryError):
+        st.sample(s, lg, [SP(), SP()], [a, b])
+    with pytest.raises(ValueError, match="twice"):
+        st.sample(s, lg, [SP(), SP()], [a, a])
+    assert st.free_pages() == 1 and st.tokens(a) == [1, 2] and s._step == 0
+    out = st.sample(s, lg[:1], [SP()], [a])
+    assert st.tokens(a) == [1, 2, int(out)] and st.free_pages() == 0
+
+
 def test_paged_pack_equals_host_packing():
     rng = np.random.default_rng(12)
     V = 128256
