@@ -28,8 +28,9 @@ namespace proc {
 
 constexpr int kThreads = 512;
 constexpr int kBlocks = 3;           // per SM
-constexpr int kTile = 12288;         // most ids of a tile
-// ids of a tile that are listed (three blocks of the largest tiles share an SM's memory)
+// Most ids of a tile, and ids of it that are listed: three blocks of the largest tiles share an SM's memory.
+template <typename In>
+constexpr int kTile = sizeof(In) == 4 ? 12288 : 16384;
 template <typename In>
 constexpr int kHits = sizeof(In) == 4 ? 1280 : 4096;
 constexpr int kPre = 4;       // history entries per thread that are in flight at a time
@@ -597,13 +598,14 @@ template <typename In, typename Out, bool kInPlace>
 cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
   // Every tile of a row reads the row's history and waits for its loads in turn, so a row has as few tiles as
   // possible; where all blocks fit on the GPU at once, as many as do.  (256 rows of 128256 fp32 with histories
-  // of about 1088: 46 us in 11 tiles, 62 in 21.)  All tiles are of one width, a multiple of 32: a tile starts on a mask word.
-  const int64_t least = (a.vocab_size + kTile - 1) / kTile;
+  // of about 1088: 46 us in 11 tiles, 62 in 21; 1024 rows of bf16: 89 us in 8 tiles, 106 in 11.)  All tiles are of
+  // one width, a multiple of 32: a tile starts on a mask word.
+  const int64_t least = (a.vocab_size + kTile<In> - 1) / kTile<In>;
   const int64_t fit = std::min<int64_t>(148 * kBlocks / a.num_rows, a.vocab_size / 2048);
   const int64_t wanted = std::max(least, fit);
   const int width = (int)((a.vocab_size + wanted - 1) / wanted + 31) / 32 * 32;
   const int tiles = (a.vocab_size + width - 1) / width;
-  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(kTile * 2 + kHits<In> * 2 + (kInPlace ? 0 : kTile * (int)sizeof(In) + 16));
+  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(kTile<In> * 2 + kHits<In> * 2 + (kInPlace ? 0 : kTile<In> * (int)sizeof(In) + 16));
   if (e != cudaSuccess) return e;
   const int bytes = width * 2 + kHits<In> * 2 + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
   tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles, width);
@@ -653,7 +655,7 @@ extern "C" int ns_process_logits(const NsProcessArgs* args, void* stream) {
   if (a.allowed && !a.allowed_rows && a.num_masks < a.num_rows)
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: fewer masks than num_rows and no allowed_rows");
   if (a.reserved != 0) return fail(NS_ERR_INVALID_ARG, "ns_process_logits: reserved must be 0");
-  const int64_t blocks = (int64_t)((a.vocab_size + proc::kTile - 1) / proc::kTile) * a.num_rows;
+  const int64_t blocks = (int64_t)((a.vocab_size + proc::kTile<float> - 1) / proc::kTile<float>) * a.num_rows;
   if (blocks > 0x7fffffff - proc::kHelpers) return fail(NS_ERR_UNSUPPORTED, "ns_process_logits: num_rows * vocab_size is too large");
 
   const int64_t in_size = a.logits_dtype == NS_DTYPE_F32 ? 4 : 2, out_size = a.out_dtype == NS_DTYPE_F32 ? 4 : 2;
