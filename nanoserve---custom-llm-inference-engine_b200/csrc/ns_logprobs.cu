@@ -7,8 +7,8 @@
 //
 // One pass over the logits gives every sum: a cluster of C blocks takes a row
 // (C by the number of rows, so that few rows still fill the GPU), each block a
-// contiguous slice of it, each thread every 256th 16-byte vector of the slice
-// (its bucket).  A thread keeps the maxima of its batches, its sum of
+// contiguous slice of it, each thread every 256th (or 128th) 16-byte vector of the
+// slice (its bucket).  A thread keeps the maxima of its batches, its sum of
 // exponentials over a reference that follows the maximum in steps, and its count
 // of larger logits.  The n largest are then in few batches: those whose maximum
 // reaches a bound that n buckets reach.  Only these are read again (out of L2);
@@ -37,8 +37,6 @@ int fail(int code, const std::string& msg);
 
 namespace lp {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;     // the portable limit
 constexpr float kLag = 8.0f;       // the reference follows the maximum in steps of at least this
 constexpr float kHuge = 0x1p100f;  // beyond it the fused argument of the exponential could overflow
@@ -46,7 +44,6 @@ constexpr int kEntries = 32;       // maxima that a thread keeps
 constexpr int kListed = 512;       // entries that are read again
 constexpr int kCands = 256;        // candidates that are ranked by counting
 typedef unsigned long long u64;
-static_assert(kMaxCluster * NS_MAX_TOP_LOGPROBS <= kThreads, "every thread ranks one key of the cluster's");
 
 // Larger value first, then smaller id, as one key to maximise; -0 counts as 0, and
 // masked elements (-inf) have key 0: they are the last to be taken, by id.
@@ -237,8 +234,12 @@ struct Part {  // a block's sums over its slice
   int count;
 };
 
-template <typename In>
-__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArgs a, int C) {
+// kThreads: 256, or less where a block takes a whole short row (then without a cluster).
+template <typename In, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_kernel(const NsLogprobArgs a, int clusters) {
+  constexpr int kWarps = kThreads / 32, kMaxCluster = kThreads < 256 ? 1 : lp::kMaxCluster;
+  static_assert(kMaxCluster == 1 || kMaxCluster * NS_MAX_TOP_LOGPROBS <= kThreads, "a thread ranks one key");
+  const int C = kMaxCluster == 1 ? 1 : clusters;
   using R = Row<In>;
   using Vec = typename R::Vec;
   constexpr int kVec = R::kVec, kUnroll = R::kUnroll;
@@ -246,12 +247,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
   __shared__ double s_sum[kWarps];
   __shared__ int s_cnt[kWarps];
   __shared__ uint32_t s_entry[kEntries][kThreads];
-  __shared__ uint32_t s_few[kWarps], s_bound;
+  __shared__ uint32_t s_few[kWarps];
   __shared__ uint16_t s_list[kListed];
   __shared__ int s_listed, s_cands;
   __shared__ u64 s_best[kThreads];  // sorted keys: the warps', then the block's, then the row's
   __shared__ u64 s_cand[kCands];
-  __shared__ u64 s_remote[(kMaxCluster - 1) * NS_MAX_TOP_LOGPROBS];  // the other blocks' keys and parts
+  __shared__ u64 s_remote[kMaxCluster * NS_MAX_TOP_LOGPROBS];  // the other blocks' keys and parts
   __shared__ Part s_part[kMaxCluster];
   if (C > 1) cluster_arrive_relaxed();  // this block runs: its shared memory may be written
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -373,16 +374,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) bound = n == 1 ? max(bound, s_few[w]) : min(bound, s_few[w]);
     if (n > 1 && bound == 0) {
-      // A warp has fewer buckets with anything in them than it should: the n-th largest of all buckets (0 if there
-      // are fewer).
-      s_best[tid] = bucket;
-      if (tid == 0) s_bound = 0;
-      __syncthreads();
-      int more = 0, same = 0;
-      for (int j = 0; j < kThreads; ++j) more += s_best[j] > bucket, same += s_best[j] == bucket;
-      if (more < n && n <= more + same) s_bound = bucket;  // one value, whoever writes it
-      __syncthreads();
-      bound = s_bound;
+      // A warp has fewer buckets with anything in them than it should: the largest bound with 16 low bits of zero
+      // that n of all buckets reach (0 if there are fewer), bit by bit.
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t higher = bound | 1u << bit;
+        if (__syncthreads_count(bucket >= higher) >= n) bound = higher;
+      }
     }
     if (bucket && bucket >= bound)
       for (int e = 0; e < entries; ++e)
@@ -392,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
         }
     const float least = bound ? key2f(bound) : -INFINITY;
     if (odd_key && (uint32_t)(odd_key >> 32) >= bound) s_cand[atomicAdd(&s_cands, 1)] = odd_key;
+    if (tid < 32) s_best[tid] = 0;  // a slice with fewer elements leaves zeros
     __syncthreads();
     const int listed = s_listed;
     if (listed <= kListed)
@@ -410,14 +408,13 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
       }
     __syncthreads();
     const int nc = s_cands;
-    u64 mine = 0;
-    int place = 32;
     if (listed <= kListed && nc <= kCands) {
-      // few candidates: each counts the larger ones
-      if (tid < nc) {
-        mine = s_cand[tid];
-        place = 0;
+      // few candidates: each counts the larger ones, and the best n take their places
+      for (int c = tid; c < nc; c += kThreads) {
+        const u64 mine = s_cand[c];
+        int place = 0;
         for (int j = 0; j < nc; ++j) place += s_cand[j] > mine;
+        if (place < n) s_best[place] = mine;
       }
     } else {
       // many equal or close ones: sorted lists, one per warp, merged.  A bucket whose best possible key
@@ -457,13 +454,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const NsLogprobArg
           s_best[tid] = list;
         }
       }
-      if (warp == 0) mine = list, place = lane;
     }
-    // the block's best n, in order; a slice with fewer elements leaves zeros
-    __syncthreads();
-    if (tid < 32) s_best[tid] = 0;
-    __syncthreads();
-    if (place < n) s_best[place] = mine;
   }
   __syncthreads();
   Part p;
@@ -537,7 +528,14 @@ cudaError_t launch(const NsLogprobArgs& a, cudaStream_t st) {
   while (C < kMaxCluster && (int64_t)a.num_rows * C < 148 * 2 && a.vocab_size / C >= 4096) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.num_rows * C), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  // Threads per block: where the rows fill the GPU more than once, blocks of 128 have eight rows of an SM in flight
+  // in place of four, and one row's search and barriers run beside the others' loads; the longest rows and few
+  // ones want the larger block.  (Top 20 in us with 256, 128 threads: 4000 bf16 rows of 1000 ids 42, 26, of 16000
+  // 80, 53, of 128256 199, 188; 4000 fp32 rows of 128256 335, 338; 400 fp32 rows of 1000 9.0, 8.2, of 50000 24,
+  // 29.  64 threads: 29, 67, 244, 443 for the 4000 rows.)
+  const int64_t row_bytes = (int64_t)a.vocab_size * (int)sizeof(In);
+  const bool small = C == 1 && (row_bytes <= 16384 || (a.num_rows > 148 * 4 && row_bytes <= 262144));
+  cfg.blockDim = dim3(small ? 128 : 256, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -545,7 +543,7 @@ cudaError_t launch(const NsLogprobArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logprob_kernel<In>, a, C);
+  return cudaLaunchKernelEx(&cfg, small ? logprob_kernel<In, 128> : logprob_kernel<In, 256>, a, C);
 }
 
 }  // namespace lp

@@ -121,6 +121,23 @@ def test_more_top_tokens_than_are_allowed(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S,V", [(700, 9001), (600, 1474), (1300, 203), (594, 40013)])
+def test_many_short_rows(S, V, dtype):
+    """More rows than the GPU takes at once, each of another kind, with masks that leave all, some or a few."""
+    rng = np.random.default_rng(S)
+    kinds = ["peaked", "flat", "ties", "rising", "falling", "constant", "wide"]
+    x = _rows(rng, S, V, torch.float32)
+    for i, kind in enumerate(kinds):
+        x[i::len(kinds)] = _rows(rng, len(range(i, S, len(kinds))), V, torch.float32, kind)
+    for i in range(0, S, 3):
+        x[i, torch.from_numpy(rng.random(V) < rng.choice([0.5, 0.99, 1.0])).to(_dev())] = -np.inf
+    x = x.to(dtype)
+    t = rng.integers(0, V, S)
+    for n in (0, 1, 12, 32):
+        _check(NS.token_logprobs(x, torch.from_numpy(t).to(_dev()), n), x.double().cpu().numpy(), t, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("offset", [0, 1, 5])
 def test_strided_rows_and_sample_indices(dtype, offset):
     rng = np.random.default_rng(offset)
