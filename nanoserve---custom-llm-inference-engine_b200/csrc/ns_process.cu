@@ -26,8 +26,7 @@ int fail(int code, const std::string& msg);
 
 namespace proc {
 
-constexpr int kThreads = 512;
-constexpr int kBlocks = 3;           // per SM
+constexpr int kMostThreads = 512;  // of a block of tile_kernel
 // Most ids of a tile, and ids of it that are listed: three blocks of the largest tiles share an SM's memory.
 template <typename In>
 constexpr int kTile = sizeof(In) == 4 ? 12032 : 16384;
@@ -175,7 +174,8 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar) {
 // 32 bits), then bits for the prompt and for biases.
 constexpr uint32_t kHalfCount = 0x1fffu, kHalfMost = 7000, kHalfBiasTwice = 0x2000u, kHalfBias = 0x4000u,
                    kHalfPrompt = 0x8000u;
-static_assert(kHalfMost + kThreads < kHalfCount, "the count is noticed before it overflows");
+static_assert(kTile<float> <= 32 * kMostThreads && kTile<__nv_bfloat16> <= 32 * kMostThreads, "a mask word each");
+static_assert(kHalfMost + kMostThreads < kHalfCount, "the count is noticed before it overflows");
 __device__ __forceinline__ uint32_t widen(uint32_t h) {
   return (h & kHalfCount) | (h & kHalfBiasTwice ? kBiasTwice : 0u) | (h & kHalfBias ? kBias : 0u) |
          (h & kHalfPrompt ? kInPrompt : 0u);
@@ -189,15 +189,15 @@ __device__ __forceinline__ uint32_t widen(uint32_t h) {
 //
 // 256 rows of 128256 fp32 with histories of about 1088 take 45 us (263.9 MB at the
 // 6446 GB/s of a copy: 41), without histories 43; 2048 rows of 50257 under masks
-// 157 us (130); 64 bf16 rows into fp32 under masks, histories of about 2300, 22 to 24
-// us (8).  Bulk copies need no registers and few instructions; what is left is a
+// 153 us (130; 160 with the mask read where it lies); 64 bf16 rows into fp32 under masks,
+// histories of about 2300, 21 us (8; 25).  Bulk copies need no registers and few instructions; what is left is a
 // block's chain of dependent loads (offsets, ids, the tile) and barriers, about 6 us
 // during which three blocks have 144 KB on their way on each SM.  Reading and writing
 // through registers, with the named ids corrected in global memory afterwards, took
 // 88 us (histories) and 51 us (none): the corrections are partial writes to lines
 // that are on their way out.  A hash table in place of 16 bits per id took 53 us.
-template <typename In, typename Out, bool kInPlace>
-__global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
+template <typename In, typename Out, bool kInPlace, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1536 / kThreads) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
   constexpr bool kSame = sizeof(In) == sizeof(Out);
   constexpr int kVec = 16 / sizeof(In);
   extern __shared__ __align__(128) unsigned char smem[];
@@ -249,7 +249,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks) tile_kernel(const __grid_co
   }
   const int mask_words = (n + 31) / 32;
   const uint32_t mask_word = mask && tid < mask_words ? __ldg(mask + tid) : 0u;
-  static_assert(kTile<In> / 32 <= kThreads, "one mask word per thread");
   const auto allowed = [&](int i) { return !mask || ((s_mask[i >> 5] >> (i & 31)) & 1u); };
   const bool counted = r.hn || r.bn;  // the same in all threads
 
@@ -602,6 +601,18 @@ cudaError_t allow_smem(int bytes) {
   return e;
 }
 
+// A block of tile_kernel has one thread per word of its tile's mask at least.
+template <typename In, typename Out, bool kInPlace, int kThreads>
+cudaError_t launch_block(const NsProcessArgs& a, unsigned blocks, int tiles, int width, cudaStream_t st) {
+  const auto bytes = [](int w) {
+    return w * 2 + kHits<In> * 2 + mask_bytes(w) + (kInPlace ? 0 : w * (int)sizeof(In) + 16);
+  };
+  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace, kThreads>>(bytes(std::min(kTile<In>, 32 * kThreads)));
+  if (e != cudaSuccess) return e;
+  tile_kernel<In, Out, kInPlace, kThreads><<<blocks, kThreads, bytes(width), st>>>(a, tiles, width);
+  return cudaGetLastError();
+}
+
 template <typename In, typename Out, bool kInPlace>
 cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
   // Every tile of a row reads the row's history and waits for its loads in turn, so a row has as few tiles as
@@ -609,15 +620,20 @@ cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
   // of about 1088: 46 us in 11 tiles, 62 in 21; 1024 rows of bf16: 89 us in 8 tiles, 106 in 11.)  All tiles are of
   // one width, a multiple of 32: a tile starts on a mask word.
   const int64_t least = (a.vocab_size + kTile<In> - 1) / kTile<In>;
-  const int64_t fit = std::min<int64_t>(148 * kBlocks / a.num_rows, a.vocab_size / 2048);
+  const int64_t fit = std::min<int64_t>(148 * 3 / a.num_rows, a.vocab_size / 2048);
   const int64_t wanted = std::max(least, fit);
   const int width = (int)((a.vocab_size + wanted - 1) / wanted + 31) / 32 * 32;
   const int tiles = (a.vocab_size + width - 1) / width;
-  const cudaError_t e = allow_smem<tile_kernel<In, Out, kInPlace>>(kTile<In> * 2 + kHits<In> * 2 + mask_bytes(kTile<In>) + (kInPlace ? 0 : kTile<In> * (int)sizeof(In) + 16));
-  if (e != cudaSuccess) return e;
-  const int bytes = width * 2 + kHits<In> * 2 + mask_bytes(width) + (kInPlace ? 0 : width * (int)sizeof(In) + 16);
-  tile_kernel<In, Out, kInPlace><<<(unsigned)(tiles * (int64_t)a.num_rows), kThreads, bytes, st>>>(a, tiles, width);
-  return cudaGetLastError();
+  const unsigned blocks = (unsigned)(tiles * (int64_t)a.num_rows);
+  // Narrow tiles get small blocks, more of them on an SM: a block's time is its chain of loads and barriers, and more
+  // rows then wait at a time.  Where all blocks are resident anyway and have long histories to count, the count
+  // wants the threads.  (4000 fp32 rows of 2500 ids, masks, histories of 150: 45 us with 512 threads, 28 with 256,
+  // 23 with 128; of 8192 ids 60, 50 with 256; 8 rows of 2500 with histories of 800: 6.1 and 6.2, of 3000: 6.2 and
+  // 10.5.)
+  const bool narrow = blocks > 148 * 3 || a.num_history_ids <= (int64_t)a.num_rows * 1024;
+  if (narrow && width <= 32 * 128) return launch_block<In, Out, kInPlace, 128>(a, blocks, tiles, width, st);
+  if (narrow && width <= 32 * 256) return launch_block<In, Out, kInPlace, 256>(a, blocks, tiles, width, st);
+  return launch_block<In, Out, kInPlace, 512>(a, blocks, tiles, width, st);
 }
 
 template <typename T>

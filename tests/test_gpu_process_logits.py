@@ -179,6 +179,30 @@ def test_long_repetitive_histories(types, mask):
     _check(got, rows, d, types[1] or types[0])
 
 
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("types", TYPES + [(torch.float32, None), (torch.bfloat16, None)],
+                         ids=["f32", "bf16-f32", "bf16", "f32-in-place", "bf16-in-place"])
+@pytest.mark.parametrize("S,V", [(600, 77), (500, 4003), (450, 4100), (450, 8191), (200, 9001)])
+def test_many_short_rows(S, V, types, mask):
+    """More rows than are worked on at once, picked in another order, with a few long histories among them."""
+    rng = np.random.default_rng(S + V)
+    d = _step(rng, S, V, hist=30, bias=3, mask=mask)
+    d["hists"][7] = [3] * 9000 + [4] * 7100 + rng.integers(0, V, 900).tolist()
+    d["hists"][S - 1] = rng.integers(0, V, 6000).tolist()
+    d["biases"][9] = [(int(v), 0.5) for v in rng.integers(0, V, 700)]
+    x = torch.from_numpy(rng.normal(0, 3, (S + 1, V)).astype(np.float32)).to(_dev()).to(types[0])
+    kw = _device(d, V)
+    if types[1] is None:
+        x = x[1:]
+        rows = x.double().cpu().numpy()
+        got = NS.process_logits(x, out=x, **kw)
+    else:
+        idx = np.arange(S)[::-1] + 1
+        rows = x.double().cpu().numpy()[idx]
+        got = NS.process_logits(x, sample_indices=torch.from_numpy(idx.copy()).to(_dev()), out_dtype=types[1], **kw)
+    _check(got, rows, d, types[1] or types[0])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_in_place_with_a_few_long_rows_among_many(dtype):
     """Rows whose ids fit the block's table, and rows that other blocks share, in one call of over 1024 rows."""
