@@ -202,13 +202,13 @@ std::string check_plan(int64_t num_pages, const int64_t* src, const int64_t* dst
 // the row of its first position by a 32-way search of the offsets; then its lanes
 // fetch what 32 rows from there need, one each, and leave it in shared memory, and
 // every lane looks up, for each of its positions (32 apart), its row, the page
-// number and the id.  What is spent is integer work and the latency of that chain
-// of loads: places are 32-bit, and kBatch positions per lane are in flight.
+// number and the id.  Runs of empty rows are skipped by another search.  What is
+// spent is integer work and the latency of that chain of loads: places are 32-bit,
+// and four positions per lane are in flight.
 //
 // 9.4 M ids in pages of 16 take 31 us (78 MB: 12 at the 6446 GB/s of a copy), the
 // same for pages in order, with issue slots 57% and L1 60% busy.  A block per row took
 // 57 us, a warp that takes the rows of its chunk one after the other 62.
-constexpr int kBatch = 4;
 
 // A row as its positions in a chunk see it: position pos is place p = pos + shift
 // of the row (counted from the first page that the tables hold), on page
@@ -235,7 +235,7 @@ struct GatherArgs {
 // kPow2: the page size is a power of two.  kEach: positions per lane.
 template <bool kPow2, int kEach>
 __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_constant__ GatherArgs a) {
-  constexpr int kChunk = kEach * 32;
+  constexpr int kChunk = kEach * 32, kBatch = kEach < 4 ? kEach : 4;
   __shared__ RowPages s_rows[kThreads / 32][32];
   const int lane = threadIdx.x % 32;
   bool bad = false;
@@ -247,22 +247,24 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
   const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kChunk;
   const int64_t end = min(__ldg(a.offsets + a.rows), a.num_ids);
   if (first < end) {
-    // the number of rows that end at or before `first`
-    int row = 0;
-    for (int n = a.rows; n > 0;) {
-      const int step = (n + 31) / 32;
-      const int at = row + (lane + 1) * step - 1;
-      const int c = __popc(__ballot_sync(0xffffffffu, at < row + n && __ldg(a.offsets + at + 1) <= first));
-      const int left = n - c * step;
-      row += c * step;
-      n = min(step - 1, left);
-    }
+    // the first row, from `row` on, that ends behind position `pos`
+    const auto find = [&](int row, int64_t pos) {
+      for (int n = a.rows - row; n > 0;) {
+        const int step = (n + 31) / 32;
+        const int at = row + (lane + 1) * step - 1;
+        const int c = __popc(__ballot_sync(0xffffffffu, at < row + n && __ldg(a.offsets + at + 1) <= pos));
+        const int left = n - c * step;
+        row += c * step;
+        n = min(step - 1, left);
+      }
+      return row;
+    };
     const uint32_t size = (uint32_t)a.page_size;
     const int bits = 31 - __clz(size);
     const uint32_t num_pages = (uint32_t)min(a.num_pages, (int64_t)0x80000000);  // page numbers are 31 bits
     int32_t* out = a.ids + first + lane;
     RowPages* rows = s_rows[threadIdx.x / 32];
-    for (int base = row; base < a.rows; base += 32) {
+    for (int base = find(0, first); base < a.rows;) {
       const int r = min(base + lane, a.rows - 1);
       const int64_t o = __ldg(a.offsets + r) - first, e = __ldg(a.offsets + r + 1) - first;
       const int64_t table = __ldg(a.page_offsets + r), table_end = min(__ldg(a.page_offsets + r + 1), a.num_table);
@@ -283,7 +285,13 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
       const int to = (int)max((int64_t)0, min(min(all, end - first), (int64_t)kChunk));
       const int ends = __popc(__ballot_sync(0xffffffffu, e < kChunk) & (uint32_t)((1ull << n) - 1));
       const int e32 = (int)max((int64_t)-1, min(e, (int64_t)kChunk));
-      uint32_t at[kEach / 4] = {};  // a byte per position: which of the window's rows it is in
+      base += 32;
+      if (to <= from) {  // empty rows: there may be many
+        if (all >= kChunk) break;
+        base = find(base, first + max(all, (int64_t)0));
+        continue;
+      }
+      uint32_t at[(kEach + 3) / 4] = {};  // a byte per position: which of the window's rows it is in
       for (int k = 0; k < min(ends, n - 1); ++k) {
         const int x = __shfl_sync(0xffffffffu, e32, k);
 #pragma unroll
@@ -407,16 +415,19 @@ int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page
     return fail(NS_ERR_INVALID_ARG, "ns_paged_history_gather: null device pointer");
   // A warp's search costs as much as several of its positions: sixteen per lane where there are warps enough to
   // fill the GPU (9.4 M ids: 31 us against 37 with eight), eight where there are not (278 K ids: 5.5 us
-  // against 6.1).
-  const bool many = num_ids >= (int64_t)148 * 48 * 32 * 16;
-  const int64_t per_block = pages::kThreads * (many ? 16 : 8);
+  // against 6.1).  Where rows have fewer than eight ids, a warp of more positions would walk through many rows, 32 at
+  // a time: one position per lane (16384 rows of 0 or 1 ids 56 us with eight, 8 with one; of 3 to 5 ids 12, 6; of 8
+  // to 10 ids 8 with eight).
+  const bool many = num_ids >= (int64_t)148 * 48 * 32 * 16, few = num_ids / 8 < num_rows;
+  const int64_t per_block = pages::kThreads * (few ? 1 : many ? 16 : 8);
   const int64_t blocks = (num_ids + per_block - 1) / per_block;
   if (blocks > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: num_ids is too large");
   const pages::GatherArgs g = {pool, num_pages, page_size, table, num_table_pages, page_offsets, offsets,
                                num_rows, out_ids, num_ids, status};
   const bool pow2 = (page_size & (page_size - 1)) == 0;
-  const auto kernel = many ? (pow2 ? pages::gather_kernel<true, 16> : pages::gather_kernel<false, 16>)
-                           : (pow2 ? pages::gather_kernel<true, 8> : pages::gather_kernel<false, 8>);
+  const auto kernel = few    ? (pow2 ? pages::gather_kernel<true, 1> : pages::gather_kernel<false, 1>)
+                      : many ? (pow2 ? pages::gather_kernel<true, 16> : pages::gather_kernel<false, 16>)
+                             : (pow2 ? pages::gather_kernel<true, 8> : pages::gather_kernel<false, 8>);
   kernel<<<(unsigned)blocks, pages::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(g);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)

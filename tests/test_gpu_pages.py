@@ -213,6 +213,28 @@ def test_gather_with_empty_and_one_id_rows(rows, p_empty):
     assert st.item() == 0 and np.array_equal(out[: want.size].cpu().numpy(), want) and (out[want.size:] == -7).all()
 
 
+@pytest.mark.parametrize("page", [1, 5, 16])
+@pytest.mark.parametrize("rows,hi", [(1, 1), (33, 3), (513, 7), (20000, 7), (20000, 1), (6000, 15)])
+def test_gather_of_many_short_rows(page, rows, hi):
+    """Rows of a few ids each, some runs of them empty, into an array that is just long enough."""
+    rng = np.random.default_rng(rows + page)
+    lens = rng.integers(0, hi + 1, rows)
+    lens[rows // 4: rows // 2] = 0
+    lens[-1] = hi
+    need = -(-lens // page)
+    table = rng.permutation(int(need.sum())).astype(np.int32)
+    pool = rng.integers(0, 1 << 30, (table.size, page)).astype(np.int32)
+    po, ho = np.concatenate([[0], np.cumsum(need)]), np.concatenate([[0], np.cumsum(lens)])
+    row = np.repeat(np.arange(rows), lens)
+    j = np.arange(row.size) - ho[row]
+    want = pool[table[po[row] + j // page], j % page]
+    d = lambda a: torch.from_numpy(a).to(_dev())  # noqa: E731
+    out = torch.full((want.size,), -7, dtype=torch.int32, device=_dev())
+    st = torch.zeros(1, dtype=torch.int32, device=_dev())
+    NS.gather_paged_history(d(pool), d(table), d(po), d(ho), out=out, status=st)
+    assert st.item() == 0 and np.array_equal(out.cpu().numpy(), want)
+
+
 def test_gather_reports_bad_tables():
     pool = torch.arange(40, dtype=torch.int32, device=_dev()).view(10, 4)
     i64 = dict(dtype=torch.int64, device=_dev())
