@@ -411,6 +411,8 @@ int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page
     return fail(NS_ERR_INVALID_ARG, "ns_paged_history_gather: num_rows, num_pages, num_table_pages or num_ids < 0");
   if (page_size <= 0) return fail(NS_ERR_INVALID_ARG, "ns_paged_history_gather: page_size must be positive");
   if (num_rows == 0 || num_ids == 0) return NS_OK;
+  if (num_rows > 1 << 30)  // the search's row numbers stay in 32 bits
+    return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: more than 2^30 rows");
   if (!page_offsets || !offsets || !out_ids || (!pool && num_pages > 0) || (!table && num_table_pages > 0))
     return fail(NS_ERR_INVALID_ARG, "ns_paged_history_gather: null device pointer");
   // A warp's search costs as much as several of its positions: sixteen per lane where there are warps enough to

@@ -680,7 +680,8 @@ extern "C" int ns_process_logits(const NsProcessArgs* args, void* stream) {
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: fewer masks than num_rows and no allowed_rows");
   if (a.reserved != 0) return fail(NS_ERR_INVALID_ARG, "ns_process_logits: reserved must be 0");
   const int64_t blocks = (int64_t)((a.vocab_size + proc::kTile<float> - 1) / proc::kTile<float>) * a.num_rows;
-  if (blocks > 0x7fffffff - proc::kHelpers) return fail(NS_ERR_UNSUPPORTED, "ns_process_logits: num_rows * vocab_size is too large");
+  if (blocks > 1 << 30)  // row numbers and their windows stay in 32 bits
+    return fail(NS_ERR_UNSUPPORTED, "ns_process_logits: num_rows * vocab_size is too large");
 
   const int64_t in_size = a.logits_dtype == NS_DTYPE_F32 ? 4 : 2, out_size = a.out_dtype == NS_DTYPE_F32 ? 4 : 2;
   const uintptr_t i0 = reinterpret_cast<uintptr_t>(a.logits), o0 = reinterpret_cast<uintptr_t>(a.out);

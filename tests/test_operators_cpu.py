@@ -132,6 +132,18 @@ def test_gather_is_checked_on_the_host():
             cabi.ns_paged_history_gather(*args)
 
 
+def test_more_rows_than_row_numbers_hold_are_refused():
+    with pytest.raises(cabi.NsError, match="2\\^30 rows"):
+        cabi.ns_paged_history_gather(16, 4, 4, 16, 4, 16, 16, (1 << 30) + 1, 16, 4)
+    for out in (1 << 45, 4096):  # another array, and in place
+        a = cabi.NsProcessArgs()
+        for k, v in dict(logits=4096, out=out, vocab_size=1, num_logit_rows=0x7fffffff, logits_row_stride=1, out_row_stride=1,
+                         num_rows=0x7fffffff - 40).items():
+            setattr(a, k, v)
+        with pytest.raises(cabi.NsError, match="too large"):
+            cabi.ns_process_logits(a)
+
+
 def test_nothing_to_do_needs_no_gpu():
     cabi.ns_process_logits(cabi.NsProcessArgs())
     cabi.ns_token_logprobs(cabi.NsLogprobArgs())
