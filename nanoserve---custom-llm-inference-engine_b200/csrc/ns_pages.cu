@@ -229,6 +229,7 @@ struct GatherArgs {
   int rows;
   int32_t* ids;
   int64_t num_ids;
+  uint32_t row_pages;  // of 2^31 ids
   uint32_t* status;
 };
 
@@ -269,11 +270,17 @@ __global__ void __launch_bounds__(kThreads, 6) gather_kernel(const __grid_consta
       const int64_t o = __ldg(a.offsets + r) - first, e = __ldg(a.offsets + r + 1) - first;
       const int64_t table = __ldg(a.page_offsets + r), table_end = min(__ldg(a.page_offsets + r + 1), a.num_table);
       const int64_t held = max(table, (int64_t)0);
-      const int64_t shift = -o - (held - table) * size;
+      const int64_t shift = (int64_t)(0 - (uint64_t)o - ((uint64_t)held - (uint64_t)table) * size);
+      // Page offsets may be any 64-bit numbers: `far` says where a difference of them could wrap around into the
+      // tables.  A place before its row's table is negative: as 32 bits without a sign it is behind the pages of
+      // 2^31 ids, which are all that a row may have.  (16384 rows take 30.8 us, as without the two; with the smaller
+      // number of pages for all rows, in place of a choice, 32.3.)
+      const bool far = table_end < 0 || (int)(table >> 32) < -1;
+      const uint32_t most = table < 0 ? a.row_pages : 0x7fffffffu;
       RowPages mine;
       mine.list = a.pages + held;
-      mine.pages = o <= e && shift > -0x7fffffff && shift < 0x7fffffff - kChunk
-                       ? (uint32_t)max((int64_t)0, min(table_end - held, (int64_t)0x7fffffff)) : 0u;
+      mine.pages = !far && o <= e && shift > -0x40000000 && shift < 0x7fffffff - kChunk
+                       ? (uint32_t)max((int64_t)0, min(table_end - held, (int64_t)most)) : 0u;
       mine.shift = (int)shift;
       __syncwarp();
       rows[lane] = mine;
@@ -425,7 +432,7 @@ int ns_paged_history_gather(const int32_t* pool, int64_t num_pages, int32_t page
   const int64_t blocks = (num_ids + per_block - 1) / per_block;
   if (blocks > 0x7fffffff) return fail(NS_ERR_UNSUPPORTED, "ns_paged_history_gather: num_ids is too large");
   const pages::GatherArgs g = {pool, num_pages, page_size, table, num_table_pages, page_offsets, offsets,
-                               num_rows, out_ids, num_ids, status};
+                               num_rows, out_ids, num_ids, 0x7fffffffu / (uint32_t)page_size + 1, status};
   const bool pow2 = (page_size & (page_size - 1)) == 0;
   const auto kernel = few    ? (pow2 ? pages::gather_kernel<true, 1> : pages::gather_kernel<false, 1>)
                       : many ? (pow2 ? pages::gather_kernel<true, 16> : pages::gather_kernel<false, 16>)
