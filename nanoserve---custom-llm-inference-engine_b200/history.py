@@ -144,7 +144,7 @@ class StoreSampling:
                 else:
                     rp, off, ids, order = self.pack(sampling_params_list, handles, sms=_sm_count(logits.device))
                     out = sampler.sample_packed(logits, rp, off, ids, row_order=order, **kw)
-                    out = sampler._with_logprobs(out, logits, logprobs, kw.get("sample_indices"))
+                    out = sampler._with_logprobs(out, logits, logprobs, kw.get("sample_indices"), rp, off, ids)
                 if append:
                     tokens = out[0] if logprobs is not None else out
                     self.append(handles, tokens[0] if isinstance(tokens, tuple) else tokens)

@@ -211,7 +211,8 @@ class Sampler:
         ``prompt_lens[i]`` ids of row i's history are its prompt, ``allowed`` and
         ``allowed_rows`` are that function's device tensors).  With ``logprobs=n``
         the result is ``(result, TokenLogprobs)``: the log-probabilities, over the
-        processed logits before temperature and filters, of the sampled tokens
+        logits after all penalties (the repetition penalty among them), biases
+        and masks and before temperature and filters, of the sampled tokens
         and of the ``n`` most likely ones."""
         if logits.dim() != 2:
             raise ValueError("logits must be [num_seqs, vocab]")
@@ -241,7 +242,7 @@ class Sampler:
                 out = self.sample_packed(
                     logits, row_params, offsets, ids, sample_indices=sample_indices, row_order=order, **step,
                 )
-                return self._with_logprobs(out, logits, logprobs, sample_indices)
+                return self._with_logprobs(out, logits, logprobs, sample_indices, row_params, offsets, ids)
         finally:
             torch.cuda.nvtx.range_pop()
 
@@ -285,13 +286,25 @@ class Sampler:
         return self._with_logprobs(out, processed, logprobs, None)
 
     @staticmethod
-    def _with_logprobs(out, logits: torch.Tensor, logprobs: Optional[int], sample_indices: Optional[torch.Tensor]):
+    def _with_logprobs(out, logits: torch.Tensor, logprobs: Optional[int], sample_indices: Optional[torch.Tensor],
+                       row_params: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+                       ids: Optional[torch.Tensor] = None):
+        """``out``, and the log-probabilities of its tokens if they are asked for.  Histories (of the rows that the
+        sampler penalised itself, in ``row_params``) say that an fp32 copy is penalised first, as the sampler does."""
         if logprobs is None:
             return out
+        from .logits import process_logits
         from .logprobs import token_logprobs
 
         tokens = out[0] if isinstance(out, tuple) else out
-        return out, token_logprobs(logits.detach(), tokens, logprobs, sample_indices=sample_indices)
+        logits = logits.detach()
+        if ids is not None:
+            rows = row_params.view(torch.float32).view(-1, packing.ROW_DTYPE.itemsize // 4)
+            penalty = rows[:, packing.ROW_DTYPE.fields["repetition_penalty"][1] // 4].contiguous()
+            logits = process_logits(logits, sample_indices=sample_indices, history_offsets=offsets, history_ids=ids,
+                                    repetition_penalty=penalty, out_dtype=torch.float32)
+            sample_indices = None
+        return out, token_logprobs(logits, tokens, logprobs, sample_indices=sample_indices)
 
     # -- pre-packed device inputs (graph-capturable) ------------------------
     def sample_packed(
