@@ -96,7 +96,12 @@ class StoreSampling:
     (those ids in CSR order, given the arrays on the device)."""
 
     def pack(self, params: Sequence, handles: Sequence[int], sms: Optional[int] = None):
-        """Device (row_params, offsets, ids, order) for ``Sampler.sample_packed``."""
+        """Device (row_params, offsets, ids, order) for ``Sampler.sample_packed``.  As ``packing.pack``, it refuses
+        requests with presence or frequency penalties or a ``logit_bias``."""
+        packing.refuse_extended(params)
+        return self._pack(params, handles, sms)
+
+    def _pack(self, params: Sequence, handles: Sequence[int], sms: Optional[int]):
         if len(handles) != len(params):
             raise ValueError(f"{len(handles)} handles for {len(params)} sampling params")
         lengths = np.fromiter((self.length(h) for h in handles), dtype=np.int64, count=len(handles))
@@ -142,7 +147,7 @@ class StoreSampling:
                         [self.prompt_length(h) for h in handles], allowed=allowed, allowed_rows=allowed_rows,
                         logprobs=logprobs, **kw)
                 else:
-                    rp, off, ids, order = self.pack(sampling_params_list, handles, sms=_sm_count(logits.device))
+                    rp, off, ids, order = self._pack(sampling_params_list, handles, _sm_count(logits.device))
                     out = sampler.sample_packed(logits, rp, off, ids, row_order=order, **kw)
                     out = sampler._with_logprobs(out, logits, logprobs, kw.get("sample_indices"), rp, off, ids)
                 if append:
@@ -227,8 +232,7 @@ class HistoryStore(StoreSampling):
         return self.pool[start : start + n].tolist()
 
     # -- one step -----------------------------------------------------------
-    def pack(self, params: Sequence, handles: Sequence[int], sms: Optional[int] = None):
-        """Device (row_params, offsets, ids, order) for ``Sampler.sample_packed``."""
+    def _pack(self, params: Sequence, handles: Sequence[int], sms: Optional[int]):
         S = len(params)
         if len(handles) != S:
             raise ValueError(f"{len(handles)} handles for {S} sampling params")

@@ -157,7 +157,17 @@ class Packed:
 
 
 def pack(params: Sequence, histories: Sequence[Sequence[int]], vocab: int, sms: Optional[int] = None) -> Packed:
-    """Pack one step's rows; with ``sms`` (the GPU's SM count) also their row order."""
+    """Pack one step's rows; with ``sms`` (the GPU's SM count) also their row order.
+
+    ``NsRowParams`` has no place for presence and frequency penalties and biases: requests that carry some raise
+    ``ValueError``.  ``process_logits`` applies them (``pack_processing`` gives its arrays, the repetition penalty among
+    them); what is left of the requests, without penalties and histories, is then packed here."""
+    refuse_extended(params)
+    return pack_plain(params, histories, vocab, sms)
+
+
+def pack_plain(params: Sequence, histories: Sequence[Sequence[int]], vocab: int, sms: Optional[int] = None) -> Packed:
+    """``pack`` for requests that ``wants_processing`` has looked at."""
     S = len(params)
     if len(histories) < S:
         raise IndexError("history_token_ids has fewer entries than sampling_params_list")
@@ -212,6 +222,13 @@ def wants_processing(params: Sequence) -> bool:
     """Whether some request carries a presence or frequency penalty or a bias.  Every request is looked at: objects of
     one type need not have the same attributes (256 requests: 20 us)."""
     return any(any(map(getattr, params, itertools.repeat(f), itertools.repeat(None))) for f in EXTENDED_FIELDS)
+
+
+def refuse_extended(params: Sequence) -> None:
+    """ValueError where a request carries what ``NsRowParams`` cannot."""
+    if wants_processing(params):
+        raise ValueError("requests with presence or frequency penalties or a logit_bias cannot be packed for "
+                         "sample_packed: apply them with process_logits, and pack the requests without them")
 
 
 @dataclass

@@ -236,8 +236,8 @@ class Sampler:
                         sample_indices=sample_indices, allowed=allowed, allowed_rows=allowed_rows, logprobs=logprobs,
                         **step,
                     )
-                packed = packing.pack(sampling_params_list, history_token_ids, vocab,
-                                      sms=_sm_count(logits.device))
+                packed = packing.pack_plain(sampling_params_list, history_token_ids, vocab,
+                                            sms=_sm_count(logits.device))
                 row_params, offsets, ids, order = self._upload(packed, logits.device)
                 out = self.sample_packed(
                     logits, row_params, offsets, ids, sample_indices=sample_indices, row_order=order, **step,
