@@ -253,7 +253,8 @@ class Sampler:
         repetition penalty among them, biases and masks), into an fp32 copy of
         the sampled rows.  ``histories`` gives the lengths of the rows'
         histories, the host arrays to upload for the ids of the rows that need
-        them, and those ids on the device."""
+        them, and those ids on the device.  With ``return_debug`` the status holds
+        what the processing reports too (bad sample indices, ids and masks)."""
         from .logits import process_logits
 
         dev, vocab = logits.device, logits.shape[1]
@@ -280,9 +281,12 @@ class Sampler:
         row_params, order_d = given.pop("rows"), given.pop("order")
         if total:
             given["history_ids"] = histories.ids(up[len(parts):], given["history_offsets"], total)
+        status = torch.zeros(1, dtype=torch.int32, device=dev) if step.get("return_debug") else None
         processed = process_logits(logits.detach(), sample_indices=sample_indices, allowed=allowed,
-                                   allowed_rows=allowed_rows, out_dtype=torch.float32, **given)
+                                   allowed_rows=allowed_rows, out_dtype=torch.float32, status=status, **given)
         out = self.sample_packed(processed, row_params, None, None, row_order=order_d, **step)
+        if status is not None:
+            out[1]["status"].bitwise_or_(status)
         return self._with_logprobs(out, processed, logprobs, None)
 
     @staticmethod
