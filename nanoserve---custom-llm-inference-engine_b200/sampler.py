@@ -213,7 +213,15 @@ class Sampler:
         the result is ``(result, TokenLogprobs)``: the log-probabilities, over the
         logits after all penalties (the repetition penalty among them), biases
         and masks and before temperature and filters, of the sampled tokens
-        and of the ``n`` most likely ones."""
+        and of the ``n`` most likely ones.
+
+        A row that has nothing left to draw (its mask allows no token, the logits or
+        biases of those it allows are all -inf, or one of them is NaN or +inf) is
+        drawn uniformly from the whole vocabulary, as the reference draws such rows
+        (nanoserve/scheduler/sampler.py:78-80), forbidden tokens included; a greedy
+        one gets token 0, or the first NaN or +inf.  Its
+        log-probabilities are ``-log(V)`` and its rank is 1: a caller that cannot
+        rule such rows out asks for ``logprobs=0`` and looks."""
         if logits.dim() != 2:
             raise ValueError("logits must be [num_seqs, vocab]")
         if not logits.is_cuda:
