@@ -77,6 +77,15 @@ void check_opt(const c10::optional<at::Tensor>& t, const at::Device& dev, const 
   TORCH_CHECK(t->scalar_type() == st, name, " has dtype ", t->scalar_type(), ", expected ", st);
 }
 
+// A kernel has written t: autograd's graphs that saved it notice, as after torch's own in-place operations.  (Tensors
+// made in inference mode have no version.)
+void wrote(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void wrote(const c10::optional<at::Tensor>& t) {
+  if (t.has_value() && t->defined()) wrote(*t);
+}
+
 // sample(logits, sample_indices, row_params, history_offsets, history_ids,
 //        uniforms, philox_seed, philox_offset, row_offset, out,
 //        out_penalized, out_filtered, out_probs, status, row_order, kernel) -> ()
@@ -154,6 +163,8 @@ void sample_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample
   a.workspace_bytes = ws.numel();
   const int rc = ns_sample(&a, stream);
   TORCH_CHECK(rc == NS_OK, "ns_sample failed (", rc, "): ", ns_last_error());
+  wrote(out);
+  for (const auto* t : {&out_penalized, &out_filtered, &out_probs, &status}) wrote(*t);
 }
 
 void check_no_grad(const at::Tensor& t, const char* op) {
@@ -267,6 +278,25 @@ void process_logits_into(const at::Tensor& logits, const c10::optional<at::Tenso
   a.status = opt_data<uint32_t>(status);
   const int rc = ns_process_logits(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   TORCH_CHECK(rc == NS_OK, "ns_process_logits failed (", rc, "): ", ns_last_error());
+  wrote(status);
+}
+
+void process_logits_into_op(const at::Tensor& logits, const c10::optional<at::Tensor>& sample_indices,
+                            const c10::optional<at::Tensor>& history_offsets,
+                            const c10::optional<at::Tensor>& history_ids,
+                            const c10::optional<at::Tensor>& prompt_lens,
+                            const c10::optional<at::Tensor>& repetition_penalty,
+                            const c10::optional<at::Tensor>& presence_penalty,
+                            const c10::optional<at::Tensor>& frequency_penalty,
+                            const c10::optional<at::Tensor>& bias_offsets,
+                            const c10::optional<at::Tensor>& bias_ids, const c10::optional<at::Tensor>& bias_values,
+                            const c10::optional<at::Tensor>& allowed, const c10::optional<at::Tensor>& allowed_rows,
+                            const c10::optional<at::Tensor>& status, at::Tensor& out) {
+  check_no_grad(out, "process_logits");
+  process_logits_into(logits, sample_indices, history_offsets, history_ids, prompt_lens, repetition_penalty,
+                      presence_penalty, frequency_penalty, bias_offsets, bias_ids, bias_values, allowed, allowed_rows,
+                      status, out);
+  wrote(out);
 }
 
 // Rows whose elements are next to each other (a copy of columns that are not).
@@ -342,6 +372,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_op(
   a.status = opt_data<uint32_t>(status);
   const int rc = ns_token_logprobs(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   TORCH_CHECK(rc == NS_OK, "ns_token_logprobs failed (", rc, "): ", ns_last_error());
+  wrote(status);
   return result;
 }
 
@@ -403,6 +434,8 @@ void copy_pages_op(at::TensorList pools, const at::Tensor& src, const at::Tensor
   }
   TORCH_CHECK_VALUE(rc != NS_ERR_INVALID_ARG, ns_last_error());
   TORCH_CHECK(rc == NS_OK, "ns_pages_copy failed (", rc, "): ", ns_last_error());
+  if (n > 0)
+    for (const at::Tensor& t : pools) wrote(t);
 }
 
 // paged_history_gather(pool, pages, page_offsets, history_offsets, out, status) -> ()
@@ -430,6 +463,8 @@ void paged_history_gather_op(const at::Tensor& pool, const at::Tensor& pages, co
       static_cast<int32_t*>(out.data_ptr()), out.numel(), opt_data<uint32_t>(status),
       c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   TORCH_CHECK(rc == NS_OK, "ns_paged_history_gather failed (", rc, "): ", ns_last_error());
+  wrote(out);
+  wrote(status);
 }
 
 }  // namespace
@@ -462,13 +497,13 @@ TORCH_LIBRARY(nanoserve_b200, m) {
 // CPU tensors get the ops' own message
 TORCH_LIBRARY_IMPL(nanoserve_b200, CPU, m) {
   m.impl("process_logits", &process_logits_op);
-  m.impl("process_logits_", &process_logits_into);
+  m.impl("process_logits_", &process_logits_into_op);
   m.impl("token_logprobs", &token_logprobs_op);
   m.impl("copy_pages", &copy_pages_op);
   m.impl("paged_history_gather", &paged_history_gather_op);
 }
 
-// these have no gradient and say so themselves: no autograd layer to go through
+// these have no gradient and say so themselves, and say what they wrote: no autograd layer to go through
 TORCH_LIBRARY_IMPL(nanoserve_b200, Autograd, m) {
   for (const char* op : {"process_logits", "process_logits_", "token_logprobs", "copy_pages", "paged_history_gather"})
     m.impl(op, torch::CppFunction::makeFallthrough());
@@ -477,7 +512,7 @@ TORCH_LIBRARY_IMPL(nanoserve_b200, Autograd, m) {
 TORCH_LIBRARY_IMPL(nanoserve_b200, CUDA, m) {
   m.impl("sample", &sample_op);
   m.impl("process_logits", &process_logits_op);
-  m.impl("process_logits_", &process_logits_into);
+  m.impl("process_logits_", &process_logits_into_op);
   m.impl("token_logprobs", &token_logprobs_op);
   m.impl("copy_pages", &copy_pages_op);
   m.impl("paged_history_gather", &paged_history_gather_op);

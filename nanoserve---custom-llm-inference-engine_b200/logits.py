@@ -67,6 +67,7 @@ def process_logits(
 
     ``out`` may be ``logits`` itself: then only what changes is written.
     Otherwise it must not overlap them, and ``logits`` is left as it was.
+    An ``out`` that requires a gradient is refused while gradients are enabled.
     ``out_dtype`` (when ``out`` is not given) is the logits' type or float32.
     Bad ids, ranges and indices are skipped and set ``NS_STATUS_*`` bits in
     ``status`` (int32 ``[1]``).  One launch on the current stream of
