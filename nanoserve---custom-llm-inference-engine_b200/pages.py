@@ -16,8 +16,9 @@ requests.  Here:
 """
 from __future__ import annotations
 
+import contextlib
 import heapq
-from typing import Dict, List, Optional, Sequence, Tuple, Union
+from typing import Dict, Iterator, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -199,6 +200,17 @@ class PagedHistoryStore(StoreSampling):
     def _needed(self, length: int) -> int:
         return -(-length // self.page_size)
 
+    @contextlib.contextmanager
+    def _taken(self, n: int) -> Iterator[List[int]]:
+        """``n`` pages, given back if the copies that fill them fail; the store's device is current."""
+        pages = self._alloc.alloc(n)
+        try:
+            with torch.cuda.device(self.device):
+                yield pages
+        except BaseException:
+            self._alloc.free(pages)
+            raise
+
     def _new(self, request: _Request) -> int:
         h = self._next
         self._next += 1
@@ -214,10 +226,9 @@ class PagedHistoryStore(StoreSampling):
             raise IndexError(f"history token id {bad} is out of range for vocab size {self.vocab}")
         if max_new_tokens < 0:
             raise ValueError("max_new_tokens must be >= 0")
-        pages = self._alloc.alloc(self._needed(ids.size + max_new_tokens))
         n = self._needed(ids.size)
-        if n:
-            with torch.cuda.device(self.device):
+        with self._taken(self._needed(ids.size + max_new_tokens)) as pages:
+            if n:
                 rows = np.zeros((n, self.page_size), dtype=np.int32)
                 rows.reshape(-1)[: ids.size] = ids
                 at = torch.tensor(pages[:n], dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
@@ -231,9 +242,8 @@ class PagedHistoryStore(StoreSampling):
             raise ValueError("n must be >= 0")
         r = self._requests[handle]
         full, rest = divmod(r.length, self.page_size)
-        own = self._alloc.alloc(n if rest else 0)
-        if own:
-            with torch.cuda.device(self.device):
+        with self._taken(n if rest else 0) as own:
+            if own:
                 copy_pages([self.pool, *self.caches], [r.pages[full]] * n, own)
         out = []
         for i in range(n):
@@ -257,15 +267,12 @@ class PagedHistoryStore(StoreSampling):
         keep = self._needed(length)
         kept, gone = r.pages[:keep], r.pages[keep:]
         if length % self.page_size and self._alloc.users(kept[-1]) > 1:
-            mine = next((p for p in gone if self._alloc.users(p) == 1), None)
-            if mine is None:
-                mine = self._alloc.alloc(1)[0]
-            else:
-                gone.remove(mine)
-            with torch.cuda.device(self.device):
-                copy_pages([self.pool, *self.caches], [kept[-1]], [mine])
-            gone.append(kept[-1])
-            kept[-1] = mine
+            mine = [p for p in gone if self._alloc.users(p) == 1][:1]
+            with self._taken(1 - len(mine)) as new:
+                own = (mine + new)[0]
+                copy_pages([self.pool, *self.caches], [kept[-1]], [own])
+            gone = [p for p in gone if p != own] + [kept[-1]]
+            kept[-1] = own
         self._alloc.free(gone)
         r.pages, r.length, r.prompt = kept, int(length), min(r.prompt, int(length))
 
