@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_kernel(const __grid_
         store_f(out + v, __fadd_rn(penalised(j == tid ? biased : load_f(out + v), w, r.pen), value));
     });
   } else {
-    const int ranges = (a.vocab_size + kRange - 1) / kRange;
+    const int ranges = (a.vocab_size - 1) / kRange + 1;
     int64_t item = 0;  // of all rows' ranges, in order
     for (int base = 0; base < a.num_rows; base += kSparseThreads) {
       bool is_long = false;
@@ -619,11 +619,11 @@ cudaError_t launch_tiles(const NsProcessArgs& a, cudaStream_t st) {
   // possible; where all blocks fit on the GPU at once, as many as do.  (256 rows of 128256 fp32 with histories
   // of about 1088: 46 us in 11 tiles, 62 in 21; 1024 rows of bf16: 89 us in 8 tiles, 106 in 11.)  All tiles are of
   // one width, a multiple of 32: a tile starts on a mask word.
-  const int64_t least = (a.vocab_size + kTile<In> - 1) / kTile<In>;
+  const int64_t least = (a.vocab_size - 1) / kTile<In> + 1;
   const int64_t fit = std::min<int64_t>(148 * 3 / a.num_rows, a.vocab_size / 2048);
   const int64_t wanted = std::max(least, fit);
   const int width = (int)((a.vocab_size + wanted - 1) / wanted + 31) / 32 * 32;
-  const int tiles = (a.vocab_size + width - 1) / width;
+  const int tiles = (a.vocab_size - 1) / width + 1;
   const unsigned blocks = (unsigned)(tiles * (int64_t)a.num_rows);
   // Narrow tiles get small blocks, more of them on an SM: a block's time is its chain of loads and barriers, and more
   // rows then wait at a time.  Where all blocks are resident anyway and have long histories to count, the count
@@ -674,12 +674,12 @@ extern "C" int ns_process_logits(const NsProcessArgs* args, void* stream) {
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: history_offsets given without history_ids");
   if (a.bias_offsets && a.num_biases > 0 && (!a.bias_ids || !a.bias_values))
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: bias_offsets given without bias_ids and bias_values");
-  if (a.allowed && (a.num_masks < 0 || a.mask_stride < (a.vocab_size + 31) / 32))
+  if (a.allowed && (a.num_masks < 0 || a.mask_stride < (a.vocab_size - 1) / 32 + 1))
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: num_masks < 0 or mask_stride < (vocab_size + 31) / 32");
   if (a.allowed && !a.allowed_rows && a.num_masks < a.num_rows)
     return fail(NS_ERR_INVALID_ARG, "ns_process_logits: fewer masks than num_rows and no allowed_rows");
   if (a.reserved != 0) return fail(NS_ERR_INVALID_ARG, "ns_process_logits: reserved must be 0");
-  const int64_t blocks = (int64_t)((a.vocab_size + proc::kTile<float> - 1) / proc::kTile<float>) * a.num_rows;
+  const int64_t blocks = ((a.vocab_size - 1) / proc::kTile<float> + (int64_t)1) * a.num_rows;
   if (blocks > 1 << 30)  // row numbers and their windows stay in 32 bits
     return fail(NS_ERR_UNSUPPORTED, "ns_process_logits: num_rows * vocab_size is too large");
 
