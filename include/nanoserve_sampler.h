@@ -86,7 +86,8 @@ extern "C" {
 #define NS_STATUS_BAD_TOKEN_ID 0x40u    /* ns_process_logits: a bias id, ns_token_logprobs: a token
                                            id outside [0, vocab)             */
 #define NS_STATUS_BAD_ROW_RANGE 0x80u   /* ns_process_logits: a row's history or bias range is
-                                           outside its array (or longer than 2^28) */
+                                           outside its array, or longer than 2^28
+                                           (history) or 2^18 (biases)        */
 #define NS_STATUS_BAD_MASK_ROW 0x100u   /* ns_process_logits: allowed_rows[i] past the masks */
 
 /* One row's sampling parameters (32 bytes, device array [num_rows]).
@@ -253,8 +254,9 @@ int ns_history_append(int32_t* pool, int64_t pool_size, const int64_t* row_dst, 
  *
  * Bad device data is never followed out of bounds: a sample index outside the
  * logits reads row 0, a history or bias id outside [0, vocab) is skipped, a
- * range outside its array counts as empty, a mask row past the masks as none;
- * each sets its NS_STATUS_* bit. */
+ * range outside its array (or of more than 2^28 history ids or 2^18 biases)
+ * counts as empty, a mask row past the masks as none; each sets its
+ * NS_STATUS_* bit. */
 typedef struct NsProcessArgs {
   const void* logits;          /* device [num_logit_rows, row_stride]      */
   int32_t logits_dtype;        /* NS_DTYPE_*                               */

@@ -41,6 +41,10 @@ constexpr uint32_t kBias = 1u << 30;
 constexpr uint32_t kBiasTwice = 1u << 29;
 constexpr uint32_t kCount = kBiasTwice - 1;
 constexpr int64_t kMaxRowIds = 1 << 28;  // a row's counts fit below the flag bits
+// An entry of an id that a row biases twice looks for a later one, work that grows with the product of the list and
+// the vocabulary: 65536 ids twice each take 0.15 s (in place 0.29), and the 2^28 entries that a history may have would
+// take many minutes.
+constexpr int64_t kMaxRowBiases = 1 << 18;
 
 __device__ __forceinline__ float load_f(const float* p) { return *p; }
 __device__ __forceinline__ float load_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -48,11 +52,12 @@ __device__ __forceinline__ void store_f(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_f(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // [o[row], o[row+1]) of an array of `total` entries; empty (and flagged) where
-// it leaves the array or is too long to count.
-__device__ __forceinline__ int row_range(const int64_t* o, int row, int64_t total, int64_t* first, uint32_t* bad) {
+// it leaves the array or has more than `most`.
+__device__ __forceinline__ int row_range(const int64_t* o, int row, int64_t total, int64_t most, int64_t* first,
+                                         uint32_t* bad) {
   const int64_t a = __ldg(o + row), b = __ldg(o + row + 1);
   *first = a;
-  if (a >= 0 && b >= a && b <= total && b - a <= kMaxRowIds) return (int)(b - a);
+  if (a >= 0 && b >= a && b <= total && b - a <= most) return (int)(b - a);
   *first = 0;
   *bad |= NS_STATUS_BAD_ROW_RANGE;
   return 0;
@@ -85,8 +90,8 @@ __device__ __forceinline__ RowWork row_work(const NsProcessArgs& a, int row) {
   r.pen.pres = a.presence_penalty ? __ldg(a.presence_penalty + row) : 0.0f;
   r.pen.freq = a.frequency_penalty ? __ldg(a.frequency_penalty + row) : 0.0f;
   int64_t h0 = 0, b0 = 0;
-  r.hn = a.history_offsets ? row_range(a.history_offsets, row, a.num_history_ids, &h0, &r.bad) : 0;
-  r.bn = a.bias_offsets ? row_range(a.bias_offsets, row, a.num_biases, &b0, &r.bad) : 0;
+  r.hn = a.history_offsets ? row_range(a.history_offsets, row, a.num_history_ids, kMaxRowIds, &h0, &r.bad) : 0;
+  r.bn = a.bias_offsets ? row_range(a.bias_offsets, row, a.num_biases, kMaxRowBiases, &b0, &r.bad) : 0;
   r.prompt = a.prompt_lens ? __ldg(a.prompt_lens + row) : 0;
   if (r.pen.rep == 1.0f && r.pen.pres == 0.0f && r.pen.freq == 0.0f) r.hn = 0;  // nothing would change
   r.hist = a.history_ids + h0;

@@ -58,7 +58,8 @@ def process_logits(
     * ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``
       float32 ``[S]``;
     * ``bias_offsets`` int64 ``[S+1]``, ``bias_ids`` int32, ``bias_values``
-      float32: if a row names an id twice, its last entry counts;
+      float32, at most 2^18 a row (a longer list is left out, as a bad range): if
+      a row names an id twice, its last entry counts;
     * ``allowed`` int32 ``[M, >= ceil(V/32)]``: token ``v`` is allowed where bit
       ``v % 32`` of word ``v // 32`` is 1.  ``allowed_rows`` int32 ``[S]`` gives
       each row's mask, a negative one none; without it row ``i`` has mask
