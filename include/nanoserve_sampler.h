@@ -345,6 +345,9 @@ int ns_token_logprobs(const NsLogprobArgs* args, void* stream);
  * (NS_ERR_INVALID_ARG) before anything is enqueued.
  *
  * ns_pages_check: ns_pages_copy's check of the page numbers alone (host only).
+ * Pools must not overlap one another (one may be named twice); pages of more
+ * than 2^31 - 1 bytes, and lists that move more than 2^41 bytes of a pool,
+ * are refused (NS_ERR_UNSUPPORTED).
  *
  * ns_pages_copy_listed: the same copies with src and dst in DEVICE memory (one
  * launch for any count, where ns_pages_copy takes one per 3500).  A page

@@ -349,6 +349,8 @@ int check_pools(const NsPagePool* pools, int32_t num_pools, int64_t num_pages, i
                                           " has no base, no bytes or pages that overlap");
     if (pools[k].page_bytes > 0x7fffffff)
       return fail(NS_ERR_UNSUPPORTED, "ns_pages_copy: pages of more than 2^31 - 1 bytes");
+    if (count > (int64_t{0x7fffffff} * kUnits) / pools[k].page_bytes)  // its blocks, of kUnits bytes at least, in 31 bits
+      return fail(NS_ERR_UNSUPPORTED, "ns_pages_copy: more than 2^41 bytes of a pool");
   }
   return NS_OK;
 }

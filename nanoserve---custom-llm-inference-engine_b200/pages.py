@@ -53,7 +53,8 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src: Pages, d
 
     ``pools`` are CUDA tensors of any type on one device, with the page number
     as their first dimension, equally many pages, and each page contiguous
-    (pages may be strided, as one half of a ``[pages, 2, ...]`` tensor is).
+    (pages may be strided, as one half of a ``[pages, 2, ...]`` tensor is; pools must not
+    overlap one another, but for one that is named twice).
     ``src`` and ``dst`` are lists, arrays or CPU tensors of page numbers.  A page
     may be copied to several places; ``ValueError`` is raised, and nothing
     copied, where a page does not exist, is a destination twice, or is both a
