@@ -17,8 +17,9 @@
 // distributed shared memory, within the cluster.
 //
 // Measured on a B200 (V = 128256; the logits' bytes at the 6446 GB/s of a copy in
-// brackets): 4096 bf16 rows, top 1: 175 us (163); 256 fp32 rows, top 20: 33 us
-// (20); 8 fp32 rows, top 5: 10 us (0.6).  Large batches are bound by the loads,
+// brackets): 4096 bf16 rows, top 1: 176 us (163) in short runs, 187 in a loop of
+// seconds under the power cap; 256 fp32 rows, top 20: 33 us (20); 8 fp32 rows,
+// top 5: 10 us (0.6).  Large batches are bound by the loads,
 // with the exponential units two thirds busy; a few hundred rows are one wave of
 // blocks, whose search for the top tokens (about 6 us after the 20 us of loads)
 // nothing overlaps: four blocks a row in place of two took 42 us, as each block

@@ -22,8 +22,10 @@ constexpr int kMaxPools = 64;
 
 // 300 pages of 32 KB in 16 pools (315 MB read and written) take 52 us, 49 at the
 // 6446 GB/s of a copy; 32 pages 8 us, of which the launch is most.  Long lists are
-// bound by the host's check of them: 87 thousand pages of 64 bytes take 188 us, 140
-// of them the check (68 us on the device as launches of 3500 pages).
+// bound by the host's check of them: 87 thousand pages of 64 bytes take about 200 us, 140
+// of them the check (68 us on the device as launches of 3500 pages).  Pages that are
+// off the 16-byte grid move in smaller units: the 300 pages take 96 us where all
+// sizes, strides and addresses are multiples of 4 bytes, 371 where they are not.
 // A block copies kUnits units of one pool: the pool's moved pages one after the
 // other, cut into equal pieces, so that small pages share a block and large ones
 // are spread.  A thread has its four loads in flight together.

@@ -195,12 +195,15 @@ __device__ __forceinline__ uint32_t widen(uint32_t h) {
 // 256 rows of 128256 fp32 with histories of about 1088 take 45 us (263.9 MB at the
 // 6446 GB/s of a copy: 41), without histories 43; 2048 rows of 50257 under masks
 // 153 us (130; 160 with the mask read where it lies); 64 bf16 rows into fp32 under masks,
-// histories of about 2300, 21 us (8; 25).  Bulk copies need no registers and few instructions; what is left is a
-// block's chain of dependent loads (offsets, ids, the tile) and barriers, about 6 us
-// during which three blocks have 144 KB on their way on each SM.  Reading and writing
-// through registers, with the named ids corrected in global memory afterwards, took
-// 88 us (histories) and 51 us (none): the corrections are partial writes to lines
-// that are on their way out.  A hash table in place of 16 bits per id took 53 us.
+// histories of about 2300, 18 us (8; 21 replayed from a graph, and 25 with the mask
+// read where it lies).  In place under masks, which only overwrites what they forbid, element
+// by element, the 256 rows take 56 us (8), in bf16 43 (4).
+// Bulk copies need no registers and few instructions; what is left is a block's chain of
+// dependent loads (offsets, ids, the tile) and barriers, about 6 us during which three
+// blocks have 144 KB on their way on each SM.  Reading and writing through registers, with
+// the named ids corrected in global memory afterwards, took 88 us (histories) and 51 us
+// (none): the corrections are partial writes to lines that are on their way out.  A hash
+// table in place of 16 bits per id took 53 us.
 template <typename In, typename Out, bool kInPlace, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1536 / kThreads) tile_kernel(const __grid_constant__ NsProcessArgs a, int tiles, int width) {
   constexpr bool kSame = sizeof(In) == sizeof(Out);
@@ -398,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads) tile_kernel(const _
     }
   } else {
     // bf16 in, fp32 out: four elements at a time along the output's 16-byte grid, so that neighbours write
-    // neighbouring sectors (eight along the tile's took 33 us in place of 31 for 183 rows of 101344 ids, and 67 for
-    // rows of 101341 whose input and output lie differently to the grid)
+    // neighbouring sectors (183 rows of 101344 ids, or of 101341 whose input and output lie differently to the
+    // grid, take 25 us; eight along the tile's took 6 % longer for the first and more than twice as long for the second)
     const auto one = [&](int i) { store_f(out + i, allowed(i) ? load_f(x + i) : -INFINITY); };
     const int before = min(n, (int)(-reinterpret_cast<uintptr_t>(out) & 15) / 4);
     const int many = (n - before) / 4 * 4;
